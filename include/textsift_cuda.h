@@ -40,7 +40,7 @@ enum {
   TS_ERR_DEVICE = -5        /* a kernel reported an error through its device flag */
 };
 
-enum { TS_DTYPE_U8 = 0, TS_DTYPE_F16 = 1, TS_DTYPE_F32 = 2, TS_DTYPE_I32 = 3 };
+enum { TS_DTYPE_U8 = 0, TS_DTYPE_F16 = 1, TS_DTYPE_F32 = 2, TS_DTYPE_I32 = 3, TS_DTYPE_BF16 = 4 };
 
 /* TS_MODE_FAST: tensor-core GEMMs (fp16 operands, f32 accumulation) and
  * tensor-core attention.  TS_MODE_EXACT: every GEMM and the attention in the
@@ -316,6 +316,103 @@ int ts_cuda_op_rope(const uint16_t* d_x, uint16_t* d_out, const uint16_t* d_cos,
  * handle's YaRN tables. */
 int ts_cuda_op_qkv_rope(ts_cuda_t* h, uint32_t layer, const uint16_t* d_x, const uint32_t* seq_offsets,
                         uint32_t n_seqs, uint16_t* d_q, uint16_t* d_k, uint16_t* d_v, void* stream);
+
+/* ---- 8-bit floating point with a scale for each block of 128, and the
+ * router's balance (no counterpart in the reference, whose weights are int4
+ * and which trains nothing).  All pointers are device pointers unless said
+ * otherwise; every call queues its work on `stream` of the current device
+ * (NULL: the default stream), allocates nothing and does not synchronize, so
+ * calls on different streams may overlap as long as their buffers do not.
+ *
+ * The format: a row is cut into blocks of 128 values; a block's scale is
+ * s = max(a * (1/448), 2^-100) in f32, a its largest finite magnitude, and
+ * its codes are e4m3(x * r), r = 1/s rounded to f32, the product rounded to
+ * f32, then to nearest even and clamped to +-448.  A NaN keeps the NaN code
+ * 0x7F, an infinity the code of +-448.
+ *   row operand [R, C]: codes u8 [R][ldc] (ldc >= C, a multiple of 16, base
+ *     16-byte aligned; bytes past C are never used, and the quantiser may
+ *     write zeros up to the next multiple of 16), scales f32
+ *     [ceil(C/128)][lds] (lds >= R: the scales of one block of columns lie
+ *     together);
+ *   weight [E, N, K]: codes u8 [E][N][ldw], scales f32
+ *     [E][ceil(N/128)][ceil(K/128)], one for each 128 x 128 block. ---- */
+
+/* Quantise x (x_dtype TS_DTYPE_F16, BF16 or F32, [rows, cols], ldx elements
+ * between rows) to a row operand.  transpose == 0: R = rows, C = cols;
+ * transpose != 0: of x's transpose, R = cols, C = rows (the operands of a
+ * weight gradient, whose blocks run along the tokens). */
+int ts_cuda_op_quant_fp8(const void* d_x, int32_t x_dtype, uint64_t ldx, uint32_t rows, uint32_t cols,
+                         int32_t transpose, uint8_t* d_codes, uint64_t ldc, float* d_scales, uint64_t lds,
+                         void* stream);
+
+/* Lay a quantised weight out by its columns: codes [E][N][ldw] -> [E][K][ldt]
+ * (ldt >= N), scales [E][ceil(N/128)][ceil(K/128)] -> [E][ceil(K/128)]
+ * [ceil(N/128)].  Exact (blocks are square).  dX = dY . W is then
+ * ts_cuda_op_matmul_fp8 of the quantised dY with this weight. */
+int ts_cuda_op_transpose_fp8(const uint8_t* d_codes, uint64_t ldw, const float* d_scales, uint32_t E, uint32_t N,
+                             uint32_t K, uint8_t* d_codes_t, uint64_t ldt, float* d_scales_t, void* stream);
+
+/* out[m, n] = sum over blocks b of as[b, m] * ws[., b] * (sum over k in b of
+ * a[m, k] * w[n, k]) + bias[n], sums in f32.
+ *   d_a, lda, d_as, ldas: row operand [M, K];
+ *   w_block 128: d_w, ldw, d_ws a weight [E, N, K] (ldws ignored);
+ *   w_block 1: d_w, ldw, d_ws, ldws a row operand [N, K], E = 1 (a weight
+ *     gradient: a = dY transposed, w = X transposed, K the tokens);
+ *   d_bias: fp16 [E][N] or NULL;
+ *   d_seg: NULL (E = 1: every row by the one weight), or i32 [E + 1]: rows
+ *     [seg[e], seg[e+1]) are multiplied with expert e's weight; rows outside
+ *     every segment are not written, bounds are clamped to [0, M];
+ *   d_out: out_dtype TS_DTYPE_F16, BF16 or F32, [M, N], ldo elements between
+ *     rows; accumulate != 0 (F32 only) adds to what d_out holds. */
+int ts_cuda_op_matmul_fp8(const uint8_t* d_a, uint64_t lda, const float* d_as, uint64_t ldas, const uint8_t* d_w,
+                          uint64_t ldw, const float* d_ws, uint64_t ldws, int32_t w_block, const uint16_t* d_bias,
+                          const int32_t* d_seg, uint32_t E, void* d_out, int32_t out_dtype, uint64_t ldo,
+                          int32_t accumulate, uint32_t M, uint32_t N, uint32_t K, void* stream);
+
+/* The form for single tokens (M <= 16): quantises x ([M, K], x_dtype F16,
+ * BF16 or F32, ldx elements between rows) as ts_cuda_op_quant_fp8 does and
+ * multiplies it with one weight [N, K] in a single launch. */
+int ts_cuda_op_matvec_fp8(const void* d_x, int32_t x_dtype, uint64_t ldx, const uint8_t* d_w, uint64_t ldw,
+                          const float* d_ws, const uint16_t* d_bias, void* d_out, int32_t out_dtype, uint64_t ldo,
+                          uint32_t M, uint32_t N, uint32_t K, void* stream);
+
+/* The router's balance over documents packed back to back.  For document s
+ * with n_s tokens (of mask 1), counts[s, e] of whose routes go to expert e:
+ *   f[s, e] = E * counts[s, e] / (k * n_s),
+ *   prob[s, e] = mean over its tokens of softmax(logits)[e],
+ *   loss = alpha / S' * sum over s, e of f[s, e] * prob[s, e],
+ * S' the number of documents with tokens, and the gradient with regard to
+ * the logits (counts held constant), times grad_scale:
+ *   grad[t, e] = grad_scale * alpha / (S' * n_s) * p[t, e] *
+ *                (f[s, e] - sum over j of p[t, j] * f[s, j]).
+ *   d_logits: dtype F16, BF16 or F32 [T, E], ldl elements between rows;
+ *   d_idx: i32 [T, k] the experts of each token (as
+ *     ts_cuda_op_router_topk writes them; an index outside [0, E) is a route
+ *     that was dropped and is not counted);
+ *   d_mask: u8 [T] (1 = token, 0 = padding) or NULL; padding has no part in
+ *     any of it and a gradient of zero;
+ *   d_seq: i32 [n_seqs + 1], ascending, or NULL (n_seqs = 1: all T tokens);
+ *     tokens outside [seq[0], seq[n_seqs]) count as padding;
+ *   d_counts: i32 [n_seqs, E]; d_prob: f32 [n_seqs, E]; d_loss: f32 [1];
+ *   d_grad: dtype [T, E], ldg elements between rows, or NULL (not wanted);
+ *   d_work: ts_cuda_router_balance_work(n_seqs, E) bytes, 8-byte aligned, of
+ *     any content, for this call alone until it is done.
+ * A logit of -inf has probability 0; a token whose logits are all -inf has a
+ * probability and gradient of 0 everywhere; one with a NaN or +inf makes its
+ * own gradient row, its document's prob and the loss NaN.  Sums do not depend
+ * on the order in which the GPU runs, so results repeat bit for bit.
+ * Limits: E <= 1024, k <= 64, T <= 2^23. */
+size_t ts_cuda_router_balance_work(uint32_t n_seqs, uint32_t E);
+int ts_cuda_op_router_balance(const void* d_logits, int32_t dtype, uint64_t ldl, const int32_t* d_idx,
+                              const uint8_t* d_mask, const int32_t* d_seq, uint32_t n_seqs, uint32_t T, uint32_t E,
+                              uint32_t k, float alpha, float grad_scale, int32_t* d_counts, float* d_prob,
+                              float* d_loss, void* d_grad, uint64_t ldg, void* d_work, size_t work_bytes,
+                              void* stream);
+
+/* Synchronize `stream` and report the error flag of the operators above on
+ * the current device as TS_ERR_DEVICE (a bounded wait that ran out; the flag
+ * is cleared), like ts_cuda_check for the operators of a handle. */
+int ts_cuda_op_check(void* stream);
 
 /* ---- expert parallelism (BASELINE config[4]'s expert-parallel variant; the
  * reference runs one process on one device and has no counterpart) ----

@@ -18,12 +18,14 @@ TS_ERR_CUDA = -3
 TS_ERR_UNSUPPORTED = -4
 TS_ERR_DEVICE = -5
 
-TS_DTYPE_U8, TS_DTYPE_F16, TS_DTYPE_F32, TS_DTYPE_I32 = 0, 1, 2, 3
+TS_DTYPE_U8, TS_DTYPE_F16, TS_DTYPE_F32, TS_DTYPE_I32, TS_DTYPE_BF16 = 0, 1, 2, 3, 4
 TS_MODE_FAST, TS_MODE_EXACT = 0, 1
 PHASES = ("expert_gate_up", "expert_down", "qkv", "attention", "o_proj", "router", "other")
 
 P = ctypes.c_void_p
 U32 = ctypes.c_uint32
+U64 = ctypes.c_uint64
+F32 = ctypes.c_float
 I32 = ctypes.c_int32
 
 
@@ -89,6 +91,16 @@ SIGNATURES = [
     ("ts_cuda_op_rope", ctypes.c_int, [P, P, P, P, P, U32, U32, U32, P]),
     ("ts_cuda_op_qkv_rope", ctypes.c_int, [P, U32, P, P, U32, P, P, P, P]),
     ("ts_cuda_op_router_addnorm", ctypes.c_int, [P, U32, P, P, P, P, P, U32, P]),
+    # 8-bit floating point with 128-block scales, router balance
+    ("ts_cuda_op_quant_fp8", ctypes.c_int, [P, I32, U64, U32, U32, I32, P, U64, P, U64, P]),
+    ("ts_cuda_op_transpose_fp8", ctypes.c_int, [P, U64, P, U32, U32, U32, P, U64, P, P]),
+    ("ts_cuda_op_matmul_fp8", ctypes.c_int, [P, U64, P, U64, P, U64, P, U64, I32, P, P, U32, P, I32, U64, I32, U32, U32,
+                                             U32, P]),
+    ("ts_cuda_op_matvec_fp8", ctypes.c_int, [P, I32, U64, P, U64, P, P, P, I32, U64, U32, U32, U32, P]),
+    ("ts_cuda_router_balance_work", ctypes.c_size_t, [U32, U32]),
+    ("ts_cuda_op_router_balance", ctypes.c_int, [P, I32, U64, P, P, P, U32, U32, U32, U32, F32, F32, P, P, P, P, U64, P,
+                                                 ctypes.c_size_t, P]),
+    ("ts_cuda_op_check", ctypes.c_int, [P]),
     ("ts_cuda_ep_unique_id", ctypes.c_size_t, [P, ctypes.c_size_t]),
     ("ts_cuda_ep_init", ctypes.c_int, [P, I32, I32, P, ctypes.c_size_t]),
     ("ts_cuda_ep_plan", ctypes.c_int, [P, P, I32, I32, I32, P, P, P, U32, P]),
