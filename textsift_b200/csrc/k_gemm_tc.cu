@@ -823,6 +823,19 @@ bool make_act_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K
   return r == CUDA_SUCCESS;
 }
 
+bool make_codes_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t ld, uint32_t box_rows) {
+  PFN_tmapEncodeTiled enc = get_encode_fn();
+  if (!enc || rows == 0 || K == 0 || (reinterpret_cast<uintptr_t>(base) & 15u) || (ld & 15u) || ld < K) return false;
+  cuuint64_t gdim[2] = {K, rows};
+  cuuint64_t gstride[1] = {ld};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), gdim, gstride, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 // SM count of the current device (persistent grid size), cached per device
 // ordinal; devices past the cache are queried on every call.
 int num_sms() {

@@ -90,6 +90,9 @@ bool make_act_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K
 // elements, `ld` elements apart, copied in boxes of box_cols x box_rows.
 bool make_tmap_2d(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t ld, uint32_t box_cols,
                   uint32_t box_rows);
+// The same for rows of K 8-bit codes, `ld` bytes apart: boxes of 128 bytes x
+// box_rows, zeros past the end of a row.
+bool make_codes_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t ld, uint32_t box_rows);
 // Streaming multiprocessors of the current device.
 int num_sms();
 
