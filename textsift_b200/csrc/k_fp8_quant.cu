@@ -5,70 +5,79 @@
 // 2^-100), r = 1/s, code = e4m3(x * r), every f32 step rounded to nearest.
 #include "ts_fp8.cuh"
 
-#include <algorithm>
-
 namespace ts {
 
-// One warp for each (row, block of 128 columns).
+// Eight lanes for each (row, block of 128 columns), 16 values a lane: the row
+// is read and its codes are written in 16-byte pieces.  A warp takes the same
+// block of four rows, so the scales it writes lie together; consecutive warps
+// take the row's next blocks.
 template <int DT>
-__global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const Fp8QuantArgs a) {
-  using D = Fp8Type<DT>;
+__global__ void __launch_bounds__(256, 8) fp8_quant_rows_kernel(const Fp8QuantArgs a, uint32_t vec) {
+  pdl_trigger();
+  pdl_wait();
   const uint32_t nb = fp8_blocks(a.cols), lane = threadIdx.x & 31;
-  const uint64_t total = (uint64_t)a.rows * nb;
-  for (uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < total; i += (uint64_t)gridDim.x * 8) {
-    const uint32_t row = (uint32_t)(i / nb), b = (uint32_t)(i % nb);
-    const auto* x = reinterpret_cast<const typename D::T*>(a.x) + row * a.ldx;
-    float v[4], m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const uint32_t c = b * kFp8Block + lane * 4 + j;
-      v[j] = c < a.cols ? D::up(x[c]) : 0.0f;
-      m = fmaxf(m, fp8_mag(v[j]));
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const float s = fp8_scale(m), r = fp8_inverse(s);
-    if (lane == 0) a.scales[b * a.lds + row] = s;
-    const uint32_t c4 = fp8_codes2(v[0], v[1], r) | fp8_codes2(v[2], v[3], r) << 16;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const uint32_t c = b * kFp8Block + lane * 4 + j;
-      if (c < a.cols) a.codes[row * a.ldc + c] = (uint8_t)(c4 >> 8 * j);
-    }
-  }
+  const uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint64_t row = i / nb * 4 + (lane >> 3);
+  const uint32_t b = (uint32_t)(i % nb), c = b * kFp8Block + (lane & 7) * 16;
+  if (row >= a.rows) return;
+  Fp8Piece<DT> p;
+  p.load(reinterpret_cast<const typename Fp8Type<DT>::T*>(a.x) + row * a.ldx, c, a.cols, vec);
+  const float s = fp8_scale(p.block_max());
+  if ((lane & 7) == 0) a.scales[b * a.lds + row] = s;
+  if (c < a.cols) *reinterpret_cast<uint4*>(a.codes + row * a.ldc + c) = p.codes(fp8_inverse(s));
 }
 
-// One block for 128 rows x 32 columns: thread (column, part) takes 16 rows.
+// A tile of 128 rows x 128 bytes (64 or 32 columns) through shared memory:
+// rows come in as they lie, and eight lanes then take one column (or, of
+// 16-bit types, two neighbours), 16 rows a lane, so that a column's 128 codes
+// leave as one line.  Four words after every 16 rows put the eight lanes'
+// rows into different banks.
 template <int DT>
-__global__ void __launch_bounds__(256) fp8_quant_cols_kernel(const Fp8QuantArgs a) {
+__global__ void __launch_bounds__(256) fp8_quant_cols_kernel(const Fp8QuantArgs a, uint32_t vec, uint32_t col_tiles) {
   using D = Fp8Type<DT>;
-  __shared__ float part[8][32];
-  const uint32_t tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const uint32_t col = blockIdx.x * 32 + tx;
-  for (uint32_t b = blockIdx.y; b < fp8_blocks(a.rows); b += gridDim.y) {
-    const auto* x = reinterpret_cast<const typename D::T*>(a.x);
-    float v[16], m = 0.0f;
+  using T = typename D::T;
+  constexpr uint32_t COLS = 128 / sizeof(T), W = sizeof(T) == 2 ? 2 : 1;  // columns a lane takes
+  constexpr uint32_t GROUP = 16 * 128 + 16;                               // bytes of 16 rows
+  __shared__ __align__(16) uint8_t tile[8 * GROUP];
+  pdl_trigger();
+  pdl_wait();
+  const uint32_t b = blockIdx.x / col_tiles, c0 = blockIdx.x % col_tiles * COLS;
+  const T* x = reinterpret_cast<const T*>(a.x);
 #pragma unroll
-    for (int j = 0; j < 16; j++) {
-      const uint32_t row = b * kFp8Block + ty * 16 + j;
-      v[j] = row < a.rows && col < a.cols ? D::up(x[row * a.ldx + col]) : 0.0f;
-      m = fmaxf(m, fp8_mag(v[j]));
+  for (uint32_t j = 0; j < 4; j++) {
+    const uint32_t r = j * 32 + (threadIdx.x >> 3), o = (threadIdx.x & 7) * 16;
+    const uint32_t c = c0 + o / sizeof(T);
+    const uint64_t row = (uint64_t)b * kFp8Block + r;
+    uint8_t* dst = tile + (r >> 4) * GROUP + (r & 15) * 128 + o;
+    constexpr uint32_t PER = 16 / sizeof(T);
+    if (vec && row < a.rows && c + PER <= a.cols) {
+      *reinterpret_cast<uint4*>(dst) = __ldg(reinterpret_cast<const uint4*>(x + row * a.ldx + c));
+    } else {
+#pragma unroll
+      for (uint32_t l = 0; l < PER; l++)
+        reinterpret_cast<T*>(dst)[l] = row < a.rows && c + l < a.cols ? x[row * a.ldx + c + l] : D::down(0.0f);
     }
-    __syncthreads();
-    part[ty][tx] = m;
-    __syncthreads();
+  }
+  __syncthreads();
+  const uint32_t col = threadIdx.x / 8 * W, g = threadIdx.x & 7;
+  const uint8_t* src = tile + g * GROUP + col * sizeof(T);
+  Fp8Piece<DT> p[W];
 #pragma unroll
-    for (int j = 0; j < 8; j++) m = fmaxf(m, part[j][tx]);
-    const float s = fp8_scale(m), r = fp8_inverse(s);
-    if (col < a.cols) {
-      if (ty == 0) a.scales[b * a.lds + col] = s;
+  for (uint32_t j = 0; j < 16; j++) {
+    T t[W];
+    if constexpr (W == 2) *reinterpret_cast<uint32_t*>(t) = *reinterpret_cast<const uint32_t*>(src + j * 128);
+    else t[0] = *reinterpret_cast<const T*>(src + j * 128);
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        const uint32_t row = b * kFp8Block + ty * 16 + j, c2 = fp8_codes2(v[j], v[j + 1], r);
-        if (row < a.rows) a.codes[col * a.ldc + row] = (uint8_t)c2;
-        if (row + 1 < a.rows) a.codes[col * a.ldc + row + 1] = (uint8_t)(c2 >> 8);
-      }
-    }
+    for (uint32_t w = 0; w < W; w++) p[w].v[j] = D::up(t[w]);
+  }
+  const uint32_t row0 = b * kFp8Block + g * 16;
+#pragma unroll
+  for (uint32_t w = 0; w < W; w++) {
+    const float s = fp8_scale(p[w].block_max());
+    const uint64_t c = c0 + col + w;
+    if (c >= a.cols) continue;
+    if (g == 0) a.scales[b * a.lds + c] = s;
+    if (row0 < a.rows) *reinterpret_cast<uint4*>(a.codes + c * a.ldc + row0) = p[w].codes(fp8_inverse(s));
   }
 }
 
@@ -97,21 +106,31 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Rows of x can be read in 16-byte pieces.
+static uint32_t fp8_vec(const Fp8QuantArgs& a) {
+  const uint64_t bytes = a.dtype == TS_DTYPE_F32 ? 4 : 2;
+  return !(reinterpret_cast<uintptr_t>(a.x) & 15u) && a.ldx * bytes % 16 == 0;
+}
+
 cudaError_t launch_fp8_quant_rows(const Fp8QuantArgs& a, cudaStream_t st) {
-  const uint64_t warps = (uint64_t)a.rows * fp8_blocks(a.cols);
-  const uint32_t grid = (uint32_t)std::min<uint64_t>((warps + 7) / 8, 1u << 20);
-  if (a.dtype == TS_DTYPE_F16) fp8_quant_rows_kernel<TS_DTYPE_F16><<<grid, 256, 0, st>>>(a);
-  else if (a.dtype == TS_DTYPE_BF16) fp8_quant_rows_kernel<TS_DTYPE_BF16><<<grid, 256, 0, st>>>(a);
-  else fp8_quant_rows_kernel<TS_DTYPE_F32><<<grid, 256, 0, st>>>(a);
-  return cudaGetLastError();
+  const uint64_t warps = ((uint64_t)a.rows + 3) / 4 * fp8_blocks(a.cols), grid = (warps + 7) / 8;
+  if (grid > 0x7fffffffu) return cudaErrorInvalidValue;
+  const dim3 g((uint32_t)grid), t(256);
+  if (a.dtype == TS_DTYPE_F16) return launch_pdl(fp8_quant_rows_kernel<TS_DTYPE_F16>, g, t, 0, st, a, fp8_vec(a));
+  if (a.dtype == TS_DTYPE_BF16) return launch_pdl(fp8_quant_rows_kernel<TS_DTYPE_BF16>, g, t, 0, st, a, fp8_vec(a));
+  return launch_pdl(fp8_quant_rows_kernel<TS_DTYPE_F32>, g, t, 0, st, a, fp8_vec(a));
 }
 
 cudaError_t launch_fp8_quant_cols(const Fp8QuantArgs& a, cudaStream_t st) {
-  const dim3 grid((a.cols + 31) / 32, std::min(fp8_blocks(a.rows), 65535u));
-  if (a.dtype == TS_DTYPE_F16) fp8_quant_cols_kernel<TS_DTYPE_F16><<<grid, 256, 0, st>>>(a);
-  else if (a.dtype == TS_DTYPE_BF16) fp8_quant_cols_kernel<TS_DTYPE_BF16><<<grid, 256, 0, st>>>(a);
-  else fp8_quant_cols_kernel<TS_DTYPE_F32><<<grid, 256, 0, st>>>(a);
-  return cudaGetLastError();
+  const uint32_t cols = a.dtype == TS_DTYPE_F32 ? 32 : 64, col_tiles = a.cols / cols + (a.cols % cols != 0);
+  const uint64_t grid = (uint64_t)col_tiles * fp8_blocks(a.rows);
+  if (grid > 0x7fffffffu) return cudaErrorInvalidValue;
+  const dim3 g((uint32_t)grid), t(256);
+  if (a.dtype == TS_DTYPE_F16)
+    return launch_pdl(fp8_quant_cols_kernel<TS_DTYPE_F16>, g, t, 0, st, a, fp8_vec(a), col_tiles);
+  if (a.dtype == TS_DTYPE_BF16)
+    return launch_pdl(fp8_quant_cols_kernel<TS_DTYPE_BF16>, g, t, 0, st, a, fp8_vec(a), col_tiles);
+  return launch_pdl(fp8_quant_cols_kernel<TS_DTYPE_F32>, g, t, 0, st, a, fp8_vec(a), col_tiles);
 }
 
 cudaError_t launch_fp8_transpose(const uint8_t* codes, uint64_t ldw, const float* scales, uint32_t E, uint32_t N,

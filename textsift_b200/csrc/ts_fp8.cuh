@@ -59,4 +59,56 @@ __device__ __forceinline__ __half2 fp8_pair(uint16_t c) {
 }
 __device__ __forceinline__ float fp8_value(uint8_t c) { return __low2float(fp8_pair(c)); }
 
+// 16 values of a row (or column) of type DT: eight lanes hold one block of 128.
+template <int DT>
+struct Fp8Piece {
+  float v[16];
+
+  // Largest magnitude over the block's eight lanes.  fmaxf passes over a NaN;
+  // only an infinity needs the second look that leaves it out.
+  __device__ __forceinline__ float block_max() const {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; j++) m = fmaxf(m, fabsf(v[j]));
+    m = lanes_max(m);
+    if (!(m < __int_as_float(0x7f800000))) {  // the same for all eight lanes
+      m = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; j++) m = fmaxf(m, fp8_mag(v[j]));
+      m = lanes_max(m);
+    }
+    return m;
+  }
+  static __device__ __forceinline__ float lanes_max(float m) {
+    const uint32_t mask = 0xffu << (threadIdx.x & 24u);
+#pragma unroll
+    for (int d = 4; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, d));
+    return m;
+  }
+  __device__ __forceinline__ uint4 codes(float r) const {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      w[j] = fp8_codes2(v[4 * j], v[4 * j + 1], r) | fp8_codes2(v[4 * j + 2], v[4 * j + 3], r) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // values i .. i + 15 of a row of n, zeros past its end
+  __device__ __forceinline__ void load(const typename Fp8Type<DT>::T* x, uint32_t i, uint32_t n, bool vec) {
+    using T = typename Fp8Type<DT>::T;
+    if (vec && i + 16 <= n) {
+      constexpr int PER = 16 / (int)sizeof(T);
+#pragma unroll
+      for (int j = 0; j < 16 / PER; j++) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x + i) + j);
+        const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int l = 0; l < PER; l++) v[j * PER + l] = Fp8Type<DT>::up(t[l]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++) v[j] = i + j < n ? Fp8Type<DT>::up(x[i + j]) : 0.0f;
+    }
+  }
+};
+
 }  // namespace ts
