@@ -439,6 +439,13 @@ cudaError_t launch_fp8_matmul(const Fp8MmArgs& a, cudaStream_t st) {
     else fp8_empty_sum_kernel<TS_DTYPE_F32><<<grid, 256, 0, st>>>(a);
     return cudaGetLastError();
   }
+  if (a.M <= kFp8MatvecRows && a.w_block != 1 && !a.seg) {
+    Fp8MvArgs v;
+    v.x = a.a; v.x_dtype = TS_DTYPE_U8; v.ldx = a.lda; v.xs = a.as; v.ldxs = a.ldas; v.w = a.w; v.ldw = a.ldw;
+    v.ws = a.ws; v.bias = a.bias; v.out = a.out; v.out_dtype = a.out_dtype; v.ldo = a.ldo; v.accumulate = a.accumulate;
+    v.M = a.M; v.N = a.N; v.K = a.K;
+    return launch_fp8_matvec(v, st);
+  }
   CUtensorMap ta, tw;
   if (!make_codes_tmap(&ta, a.a, a.M, a.K, a.lda, f8::BM) ||
       !make_codes_tmap(&tw, a.w, (uint64_t)a.E * a.N, a.K, a.ldw, f8::W_BOX))
@@ -457,58 +464,6 @@ cudaError_t launch_fp8_matmul(const Fp8MmArgs& a, cudaStream_t st) {
   if (fills(256)) return launch_gemm_out<256, 128>(ta, tw, a, m_tiles, st);
   if (fills(128)) return launch_gemm_out<128, 128>(ta, tw, a, m_tiles, st);
   return launch_gemm_out<64, 128>(ta, tw, a, m_tiles, st);
-}
-
-// One warp for each output row n of the weight and row m of x: lane l takes
-// the values l, l + 32, ... of a block, quantises them and multiplies.
-template <int XT, int OT>
-__global__ void __launch_bounds__(256) fp8_matvec_simt_kernel(const Fp8MvArgs a) {
-  using X = Fp8Type<XT>;
-  using O = Fp8Type<OT>;
-  const uint32_t n = blockIdx.x * 8 + (threadIdx.x >> 5), m = blockIdx.y, lane = threadIdx.x & 31;
-  if (n >= a.N) return;
-  const uint32_t kb = fp8_blocks(a.K);
-  const auto* x = reinterpret_cast<const typename X::T*>(a.x) + m * a.ldx;
-  float acc = 0.0f;
-  for (uint32_t b = 0; b < kb; b++) {
-    float v[4], mx = 0.0f, part = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const uint32_t k = b * kFp8Block + j * 32 + lane;
-      v[j] = k < a.K ? X::up(x[k]) : 0.0f;
-      mx = fmaxf(mx, fp8_mag(v[j]));
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    const float s = fp8_scale(mx), r = fp8_inverse(s);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const uint32_t k = b * kFp8Block + j * 32 + lane;
-      if (k < a.K) part = fmaf(fp8_value((uint8_t)fp8_codes2(v[j], 0.0f, r)), fp8_value(a.w[n * a.ldw + k]), part);
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
-    acc = fmaf(part, s * a.ws[(uint64_t)(n / kFp8Block) * kb + b], acc);
-  }
-  if (lane == 0) {
-    if (a.bias) acc += __half2float(reinterpret_cast<const __half*>(a.bias)[n]);
-    (reinterpret_cast<typename O::T*>(a.out) + m * a.ldo)[n] = O::down(acc);
-  }
-}
-
-template <int XT>
-static void launch_mv(const Fp8MvArgs& a, cudaStream_t st) {
-  const dim3 grid((a.N + 7) / 8, a.M);
-  if (a.out_dtype == TS_DTYPE_F16) fp8_matvec_simt_kernel<XT, TS_DTYPE_F16><<<grid, 256, 0, st>>>(a);
-  else if (a.out_dtype == TS_DTYPE_BF16) fp8_matvec_simt_kernel<XT, TS_DTYPE_BF16><<<grid, 256, 0, st>>>(a);
-  else fp8_matvec_simt_kernel<XT, TS_DTYPE_F32><<<grid, 256, 0, st>>>(a);
-}
-
-cudaError_t launch_fp8_matvec(const Fp8MvArgs& a, cudaStream_t st) {
-  if (a.x_dtype == TS_DTYPE_F16) launch_mv<TS_DTYPE_F16>(a, st);
-  else if (a.x_dtype == TS_DTYPE_BF16) launch_mv<TS_DTYPE_BF16>(a, st);
-  else launch_mv<TS_DTYPE_F32>(a, st);
-  return cudaGetLastError();
 }
 
 }  // namespace ts

@@ -53,10 +53,14 @@ struct Fp8MmArgs {
 };
 cudaError_t launch_fp8_matmul(const Fp8MmArgs& a, cudaStream_t st);
 
+// x of a floating type, quantised on the way, or codes (x_dtype TS_DTYPE_U8)
+// with their scales xs.
 struct Fp8MvArgs {
   const void* x = nullptr;
   int x_dtype = 0;
   uint64_t ldx = 0;
+  const float* xs = nullptr;
+  uint64_t ldxs = 0;
   const uint8_t* w = nullptr;
   uint64_t ldw = 0;
   const float* ws = nullptr;
@@ -64,6 +68,7 @@ struct Fp8MvArgs {
   void* out = nullptr;
   int out_dtype = 0;
   uint64_t ldo = 0;
+  int accumulate = 0;
   uint32_t M = 0, N = 0, K = 0;
 };
 cudaError_t launch_fp8_matvec(const Fp8MvArgs& a, cudaStream_t st);
