@@ -88,9 +88,12 @@ struct BalanceArgs {
   void* grad = nullptr;
   uint64_t ldg = 0;
   void* work = nullptr;
+  uint32_t loss_blocks = 1;  // set by the launcher
 };
 constexpr uint32_t kBalanceMaxExperts = 1024, kBalanceMaxK = 64, kBalanceMaxTokens = 1u << 23;
+// Calls of at most this many logits run as one cluster.
+constexpr uint64_t kBalanceClusterLogits = 1u << 17;
 size_t balance_work_bytes(uint32_t S, uint32_t E);
-cudaError_t launch_router_balance(const BalanceArgs& a, cudaStream_t st);
+cudaError_t launch_router_balance(BalanceArgs a, cudaStream_t st);
 
 }  // namespace ts
