@@ -9,27 +9,31 @@
 // Probabilities are summed as 64-bit integers in units of 2^-40 across blocks:
 // integer sums do not depend on the order of the atomics, 2^23 tokens stay
 // below 2^63, and a term's rounding error is 2^-41.  Inside a block they are
-// f32 sums of at most 16 tokens a lane in a fixed order.
+// f32 sums of at most MAX_RUN tokens a lane in a fixed order.
 //
-// Four phases (clear, count, tokens, loss), each written for `nb` blocks:
-// four launches for large calls, or one cluster of eight blocks with the
-// cluster's barrier between phases, where launches cost more than they do.
+// Large calls run as four launches (clear, count, tokens, loss), small ones
+// as one block that keeps counts and sums in shared memory: there the chain
+// of launches and of global round trips is all that costs.
 #include "ts_fp8.cuh"
+#include "ts_kernels.h"
 
 #include <algorithm>
 
 namespace ts {
 
 namespace bal {
-constexpr uint32_t THREADS = 256, WARPS = 8, CLUSTER = 8;
+constexpr uint32_t THREADS = 256, WARPS = 8;
 constexpr uint32_t COUNT_TOKENS = 256;  // tokens of a counting tile
-constexpr uint32_t RUN = 4;             // tokens a lane group takes in a row
-constexpr uint32_t MAX_LOSS_BLOCKS = 128;
+constexpr uint32_t MAX_RUN = 16;        // most tokens a lane group takes in a row
+constexpr uint32_t SEQ_SMEM = 1024;     // document offsets that a block keeps in shared memory
+constexpr uint32_t MAX_LOSS_BLOCKS = 256;
 constexpr float UNIT = 1099511627776.0f;  // 2^40
+// the one-block form
+constexpr uint32_t ONE_THREADS = 1024, ONE_TABLE = 4096, ONE_TOKENS = 1024;
 }  // namespace bal
 
 static uint32_t balance_loss_blocks(uint32_t S, uint32_t E) {
-  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(bal::MAX_LOSS_BLOCKS, (uint64_t)S * E / 1024));
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(bal::MAX_LOSS_BLOCKS, (uint64_t)S * E / bal::THREADS));
 }
 
 // Work area: sums u64 [S][E], partial losses f64 [blocks], tokens i32 [S],
@@ -56,18 +60,32 @@ size_t balance_work_bytes(uint32_t S, uint32_t E) {
   return (size_t)S * E * 8 + balance_loss_blocks(S, E) * 8 + (size_t)S * 8 + 12;
 }
 
-// The document of token t, or -1: padding, or outside [seq[0], seq[S]).
-__device__ __forceinline__ int balance_doc(const BalanceArgs& a, uint32_t t) {
-  if (a.mask && !a.mask[t]) return -1;
-  if (!a.seq) return 0;
-  if ((int)t < a.seq[0] || (int)t >= a.seq[a.S]) return -1;
-  uint32_t lo = 0, hi = a.S;  // seq[lo] <= t < seq[hi]
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (a.seq[mid] <= (int)t) lo = mid;
-    else hi = mid;
+// Document offsets as a block sees them: in shared memory when there are few.
+struct BalanceSeq {
+  const int* at;  // null: one document of all tokens
+  uint32_t S;
+  // The document of token t, or -1: padding, or outside [seq[0], seq[S]).
+  __device__ __forceinline__ int doc(const BalanceArgs& a, uint32_t t) const {
+    if (a.mask && !a.mask[t]) return -1;
+    if (!at) return 0;
+    if ((int)t < at[0] || (int)t >= at[S]) return -1;
+    uint32_t lo = 0, hi = S;  // at[lo] <= t < at[hi]
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (at[mid] <= (int)t) lo = mid;
+      else hi = mid;
+    }
+    return (int)lo;
   }
-  return (int)lo;
+};
+// Copies the offsets into `room` where they fit; the caller synchronizes.
+__device__ __forceinline__ BalanceSeq balance_seq(const BalanceArgs& a, int* room, uint32_t size) {
+  BalanceSeq q{a.seq, a.S};
+  if (a.seq && a.S < size) {
+    for (uint32_t i = threadIdx.x; i <= a.S; i += blockDim.x) room[i] = a.seq[i];
+    q.at = room;
+  }
+  return q;
 }
 
 // True in every thread of the block that is the last of nb to come here; what
@@ -82,61 +100,66 @@ __device__ __forceinline__ bool balance_last(unsigned* ticket, uint32_t nb) {
   return got == nb - 1;
 }
 
-__device__ __forceinline__ void balance_clear(const BalanceArgs& a, uint32_t bid, uint32_t nb) {
+// Each of these kernels waits for the work before it and only then lets the
+// next one start, so that a kernel of the chain may read the caller's inputs
+// (though not what the chain writes) before its own wait.
+__global__ void __launch_bounds__(bal::THREADS) balance_clear_kernel(const BalanceArgs a) {
+  pdl_wait();
+  pdl_trigger();
   const BalanceWork w = balance_work(a);
-  const uint64_t step = (uint64_t)nb * bal::THREADS;
-  for (uint64_t i = bid * bal::THREADS + threadIdx.x; i < (uint64_t)a.S * a.E; i += step) {
+  const uint64_t step = (uint64_t)gridDim.x * bal::THREADS;
+  for (uint64_t i = (uint64_t)blockIdx.x * bal::THREADS + threadIdx.x; i < (uint64_t)a.S * a.E; i += step) {
     w.sum[i] = 0;
     a.counts[i] = 0;
   }
-  for (uint64_t i = bid * bal::THREADS + threadIdx.x; i < 2ull * a.S + 3; i += step) w.tokens[i] = 0;
+  for (uint64_t i = (uint64_t)blockIdx.x * bal::THREADS + threadIdx.x; i < 2ull * a.S + 3; i += step) w.tokens[i] = 0;
 }
 
-// Counts of tiles of 256 tokens: through shared memory where the tile lies in
+// Counts of a tile of 256 tokens: through shared memory where the tile lies in
 // one document, straight to the document's row where it does not.  The last
 // block counts the documents that have tokens.
-__device__ __forceinline__ void balance_count(const BalanceArgs& a, uint32_t bid, uint32_t nb) {
+__global__ void __launch_bounds__(bal::THREADS) balance_count_kernel(const BalanceArgs a) {
   using namespace bal;
   __shared__ int hist[kBalanceMaxExperts];
   __shared__ int doc[COUNT_TOKENS];
+  __shared__ int room[SEQ_SMEM];
+  __shared__ int top[WARPS];
   const BalanceWork w = balance_work(a);
-  for (uint32_t t0 = bid * COUNT_TOKENS; t0 < a.T; t0 += nb * COUNT_TOKENS) {
-    const uint32_t t = t0 + threadIdx.x, n = min(COUNT_TOKENS, a.T - t0);
-    const int s = t < a.T ? balance_doc(a, t) : -1;
-    doc[threadIdx.x] = s;
-    for (uint32_t e = threadIdx.x; e < a.E; e += THREADS) hist[e] = 0;
-    // the tile's one document: the largest of all, equal to every one that is not padding
-    int one = s;
+  const BalanceSeq q = balance_seq(a, room, SEQ_SMEM);
+  __syncthreads();
+  const uint32_t t0 = blockIdx.x * COUNT_TOKENS, t = t0 + threadIdx.x, n = min(COUNT_TOKENS, a.T - t0);
+  const int s = t < a.T ? q.doc(a, t) : -1;
+  doc[threadIdx.x] = s;
+  for (uint32_t e = threadIdx.x; e < a.E; e += THREADS) hist[e] = 0;
+  // the tile's one document: the largest of all, equal to every one that is not padding
+  int one = s;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) one = max(one, __shfl_xor_sync(0xffffffffu, one, d));
-    __shared__ int top[WARPS];
-    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = one;
-    __syncthreads();
-    for (uint32_t i = 0; i < WARPS; i++) one = max(one, top[i]);
-    const bool single = __syncthreads_and(s < 0 || s == one);
-    const int live = __syncthreads_count(s >= 0);
-    if (live) {
-      if (single) {
-        if (threadIdx.x == 0) atomicAdd(&w.tokens[one], live);
-      } else if (s >= 0) {
-        atomicAdd(&w.tokens[s], 1);
-      }
-      for (uint32_t r = threadIdx.x; r < n * a.k; r += THREADS) {
-        const int d = doc[r / a.k];
-        if (d < 0) continue;
-        const int e = a.idx[(uint64_t)t0 * a.k + r];
-        if (e < 0 || e >= (int)a.E) continue;
-        if (single) atomicAdd(&hist[e], 1);
-        else atomicAdd(&a.counts[(uint64_t)d * a.E + e], 1);
-      }
-      __syncthreads();
-      if (single)
-        for (uint32_t e = threadIdx.x; e < a.E; e += THREADS)
-          if (hist[e]) atomicAdd(&a.counts[(uint64_t)one * a.E + e], hist[e]);
+  for (int d = 16; d; d >>= 1) one = max(one, __shfl_xor_sync(0xffffffffu, one, d));
+  if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = one;
+  __syncthreads();
+  for (uint32_t i = 0; i < WARPS; i++) one = max(one, top[i]);
+  const bool single = __syncthreads_and(s < 0 || s == one);
+  const int live = __syncthreads_count(s >= 0);
+  pdl_wait();
+  pdl_trigger();
+  if (live) {
+    if (single) {
+      if (threadIdx.x == 0) atomicAdd(&w.tokens[one], live);
+    } else if (s >= 0) {
+      atomicAdd(&w.tokens[s], 1);
+    }
+    for (uint32_t r = threadIdx.x; r < n * a.k; r += THREADS) {
+      const int d = doc[r / a.k], e = __ldg(&a.idx[(uint64_t)t0 * a.k + r]);
+      if (d < 0 || e < 0 || e >= (int)a.E) continue;
+      if (single) atomicAdd(&hist[e], 1);
+      else atomicAdd(&a.counts[(uint64_t)d * a.E + e], 1);
     }
     __syncthreads();
+    if (single)
+      for (uint32_t e = threadIdx.x; e < a.E; e += THREADS)
+        if (hist[e]) atomicAdd(&a.counts[(uint64_t)one * a.E + e], hist[e]);
   }
-  if (balance_last(&w.ticket[0], nb)) {
+  if (balance_last(&w.ticket[0], gridDim.x)) {
     int used = 0;
     for (uint32_t s0 = 0; s0 < a.S; s0 += THREADS)
       used += __syncthreads_count(s0 + threadIdx.x < a.S && __ldcg(&w.tokens[min(s0 + threadIdx.x, a.S - 1)]) > 0);
@@ -144,267 +167,350 @@ __device__ __forceinline__ void balance_count(const BalanceArgs& a, uint32_t bid
   }
 }
 
-// L lanes hold a token's logits, V each, in pieces of 16 bytes: piece j of
-// lane l is the token's (j L + l)-th.  A warp takes 32 / L tokens at once and
-// RUN in a row for each lane group; the group's document, its counts and the
-// sums of its probabilities stay in registers until the document ends.
+// A token's logits in L lanes, V each, in pieces of 16 bytes: piece j of lane
+// l is the token's (j L + l)-th.
 template <int DT, int L, int V>
-__device__ __forceinline__ void balance_tokens(const BalanceArgs& a, uint32_t bid, uint32_t nb) {
-  using namespace bal;
+struct BalanceToken {
   using D = Fp8Type<DT>;
   using T = typename D::T;
-  constexpr int PER = 16 / (int)sizeof(T), GROUPS = 32 / L;
-  constexpr uint32_t TILE = WARPS * GROUPS * RUN;
-  __shared__ float red[WARPS][L * V];
-  __shared__ int red_doc[WARPS];
-  const BalanceWork w = balance_work(a);
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, grp = lane / L;
-  const uint32_t mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << (grp * L);
-  const float inf = __int_as_float(0x7f800000);
-  const bool vec_in = !(reinterpret_cast<uintptr_t>(a.logits) & 15u) && a.ldl * sizeof(T) % 16 == 0;
-  const bool vec_out = !(reinterpret_cast<uintptr_t>(a.grad) & 15u) && a.ldg * sizeof(T) % 16 == 0;
-  const float all = a.grad_scale * a.alpha * (float)a.E / (float)a.k / (float)max(__ldcg(w.docs), 1);
-  auto expert = [&](int j) { return (uint32_t)((j / PER * L + (int)l) * PER + j % PER); };
-  float cnt[V], psum[V];
-  for (uint32_t t0 = bid * TILE; t0 < a.T; t0 += nb * TILE) {
-    int held = -1;  // the document that cnt and psum belong to
-    float coef = 0.0f;
-    auto flush = [&]() {
-      if (held < 0) return;
+  static constexpr int PER = 16 / (int)sizeof(T), GROUPS = 32 / L;
+  static_assert(V % PER == 0, "whole pieces");
+  float z[V];           // logits, then probabilities
+  float scale, mean, fill;  // gradient: scale * p * (count - mean), or fill where scale is 0
+
+  static __device__ __forceinline__ uint32_t lane() { return threadIdx.x % L; }
+  static __device__ __forceinline__ uint32_t group() { return (threadIdx.x & 31) / L; }
+  static __device__ __forceinline__ uint32_t mask() {
+    return L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << (group() * L);
+  }
+  static __device__ __forceinline__ uint32_t expert(int j) {
+    return (uint32_t)((j / PER * L + (int)lane()) * PER + j % PER);
+  }
+  __device__ __forceinline__ void load(const BalanceArgs& a, uint32_t t, bool vec) {
+    const T* x = static_cast<const T*>(a.logits) + t * a.ldl;
 #pragma unroll
-      for (int j = 0; j < V; j++)
-        if (psum[j] > 0.0f) atomicAdd(&w.sum[(uint64_t)held * a.E + expert(j)], __float2ull_rn(psum[j] * UNIT));
-    };
+    for (int j = 0; j < V; j += PER) {
+      const uint32_t e = expert(j);
+      if (vec && e + PER <= a.E) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x + e));
 #pragma unroll
-    for (int j = 0; j < V; j++) psum[j] = 0.0f;
-    for (uint32_t i = 0; i < RUN; i++) {
-      const uint32_t t = t0 + (warp * RUN + i) * GROUPS + grp;
-      if (t >= a.T) break;
-      float z[V];
-      const T* x = static_cast<const T*>(a.logits) + t * a.ldl;
+        for (int i = 0; i < PER; i++) z[j + i] = D::up(reinterpret_cast<const T*>(&raw)[i]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < V; j += PER) {
-        const uint32_t e = expert(j);
-        if (vec_in && e + PER <= a.E) {
-          const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x + e));
-#pragma unroll
-          for (int i2 = 0; i2 < PER; i2++) z[j + i2] = D::up(reinterpret_cast<const T*>(&raw)[i2]);
-        } else {
-#pragma unroll
-          for (int i2 = 0; i2 < PER; i2++) z[j + i2] = e + i2 < a.E ? D::up(x[e + i2]) : -inf;
-        }
-      }
-      const int s = balance_doc(a, t);
-      float scale = 0.0f, mean = 0.0f, fill = 0.0f;
-      if (s >= 0) {
-        if (s != held) {
-          flush();
-          held = s;
-          const float n = (float)__ldcg(&w.tokens[s]);
-          coef = all / n / n;
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            psum[j] = 0.0f;
-            cnt[j] = expert(j) < a.E ? (float)__ldcg(&a.counts[(uint64_t)s * a.E + expert(j)]) : 0.0f;
-          }
-        }
-        float m = -inf;
-#pragma unroll
-        for (int j = 0; j < V; j++) m = fmaxf(m, z[j]);
-#pragma unroll
-        for (int d = L / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, d));
-        float sum = 0.0f, dot = 0.0f;
-        bool odd = false;
-        if (!(m > -inf && m < inf)) {  // +inf, or nothing but -inf and NaN
-#pragma unroll
-          for (int j = 0; j < V; j++) odd |= !(z[j] < inf);
-          odd = __any_sync(mask, odd);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            z[j] = expf(z[j] - m);
-            sum += z[j];
-            dot = fmaf(z[j], cnt[j], dot);
-          }
-#pragma unroll
-          for (int d = L / 2; d; d >>= 1) {
-            sum += __shfl_xor_sync(mask, sum, d);
-            dot += __shfl_xor_sync(mask, dot, d);
-          }
-          odd = !(sum == sum);  // a NaN among finite logits
-        }
-        if (odd) {
-          if (l == 0) w.bad[s] = 1;
-          fill = __int_as_float(0x7fc00000);
-        } else if (sum > 0.0f) {
-          const float inv = 1.0f / sum;
-          mean = dot * inv;
-          scale = coef;
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            z[j] *= inv;
-            psum[j] += z[j];
-          }
-        }
-      }
-      if (!a.grad) continue;
-      T* g = static_cast<T*>(a.grad) + t * a.ldg;
-#pragma unroll
-      for (int j = 0; j < V; j += PER) {
-        const uint32_t e = expert(j);
-        uint4 raw;
-        T* out = reinterpret_cast<T*>(&raw);
-#pragma unroll
-        for (int i2 = 0; i2 < PER; i2++)
-          out[i2] = D::down(scale != 0.0f ? scale * z[j + i2] * (cnt[j + i2] - mean) : fill);
-        if (vec_out && e + PER <= a.E) {
-          *reinterpret_cast<uint4*>(g + e) = raw;
-        } else {
-#pragma unroll
-          for (int i2 = 0; i2 < PER; i2++)
-            if (e + i2 < a.E) g[e + i2] = out[i2];
-        }
+        for (int i = 0; i < PER; i++) z[j + i] = e + i < a.E ? D::up(x[e + i]) : -__int_as_float(0x7f800000);
       }
     }
-    // one row of sums a warp where all its groups hold the same document
-    const int first = __shfl_sync(0xffffffffu, held, 0);
-    const bool same = __all_sync(0xffffffffu, held == first || held < 0) && first >= 0;
-    if (same) {
+  }
+  // Probabilities and the gradient's terms of a token of document s; adds the
+  // probabilities to psum.
+  __device__ __forceinline__ void softmax(const float (&cnt)[V], float (&psum)[V], float coef, int* bad) {
+    const float inf = __int_as_float(0x7f800000);
+    scale = mean = fill = 0.0f;
+    float m = -inf, sum = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; j++) m = fmaxf(m, z[j]);
+#pragma unroll
+    for (int d = L / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(mask(), m, d));
+    bool odd = false;
+    if (!(m > -inf && m < inf)) {  // +inf, or nothing but -inf and NaN
+#pragma unroll
+      for (int j = 0; j < V; j++) odd |= !(z[j] < inf);
+      odd = __any_sync(mask(), odd);
+    } else {
 #pragma unroll
       for (int j = 0; j < V; j++) {
-#pragma unroll
-        for (int d = L; d < 32; d <<= 1) psum[j] += __shfl_xor_sync(0xffffffffu, psum[j], d);
-        if (grp == 0) red[warp][expert(j)] = psum[j];
+        z[j] = expf(z[j] - m);
+        sum += z[j];
+        dot = fmaf(z[j], cnt[j], dot);
       }
-    } else {
-      flush();
+#pragma unroll
+      for (int d = L / 2; d; d >>= 1) {
+        sum += __shfl_xor_sync(mask(), sum, d);
+        dot += __shfl_xor_sync(mask(), dot, d);
+      }
+      odd = !(sum == sum);  // a NaN among finite logits
     }
-    if (lane == 0) red_doc[warp] = same ? first : -1;
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < a.E; e += THREADS) {
-      float sum = 0.0f;
-      for (uint32_t i = 0; i < WARPS; i++) {
-        const int s = red_doc[i];
-        if (s >= 0) sum += red[i][e];
-        if (s >= 0 && (i + 1 == WARPS || red_doc[i + 1] != s)) {
-          atomicAdd(&w.sum[(uint64_t)s * a.E + e], __float2ull_rn(sum * UNIT));
-          sum = 0.0f;
+    if (odd) {
+      if (lane() == 0) *bad = 1;
+      fill = __int_as_float(0x7fc00000);
+    } else if (sum > 0.0f) {
+      const float inv = 1.0f / sum;
+      mean = dot * inv;
+      scale = coef;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        z[j] *= inv;
+        psum[j] += z[j];
+      }
+    }
+  }
+  __device__ __forceinline__ void write(const BalanceArgs& a, uint32_t t, const float (&cnt)[V], bool vec) const {
+    T* g = static_cast<T*>(a.grad) + t * a.ldg;
+#pragma unroll
+    for (int j = 0; j < V; j += PER) {
+      const uint32_t e = expert(j);
+      uint4 raw;
+      T* out = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < PER; i++) out[i] = D::down(scale != 0.0f ? scale * z[j + i] * (cnt[j + i] - mean) : fill);
+      if (vec && e + PER <= a.E) {
+        *reinterpret_cast<uint4*>(g + e) = raw;
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+          if (e + i < a.E) g[e + i] = out[i];
+      }
+    }
+  }
+  static __device__ __forceinline__ bool vec_in(const BalanceArgs& a) {
+    return !(reinterpret_cast<uintptr_t>(a.logits) & 15u) && a.ldl * sizeof(T) % 16 == 0;
+  }
+  static __device__ __forceinline__ bool vec_out(const BalanceArgs& a) {
+    return !(reinterpret_cast<uintptr_t>(a.grad) & 15u) && a.ldg * sizeof(T) % 16 == 0;
+  }
+  // grad_scale alpha E / k for S' documents; over n twice for one of n tokens
+  static __device__ __forceinline__ float factor(const BalanceArgs& a, int docs) {
+    return a.grad_scale * a.alpha * (float)a.E / (float)a.k / (float)max(docs, 1);
+  }
+};
+
+// A warp takes 32 / L tokens at once and `run` in a row for each lane group,
+// the next token's logits loaded while one is worked on; the group's document,
+// its counts and the sums of its probabilities stay in registers until the
+// document ends.
+template <int DT, int L, int V>
+__global__ void __launch_bounds__(bal::THREADS) balance_tokens_kernel(const BalanceArgs a, uint32_t run) {
+  using namespace bal;
+  using K = BalanceToken<DT, L, V>;
+  __shared__ float red[WARPS][L * V];
+  __shared__ int red_doc[WARPS];
+  __shared__ int room[SEQ_SMEM];
+  const BalanceWork w = balance_work(a);
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool vec_in = K::vec_in(a), vec_out = K::vec_out(a);
+  const uint32_t first_t = (blockIdx.x * WARPS + warp) * run * K::GROUPS + K::group();
+  K next;
+  if (first_t < a.T) next.load(a, first_t, vec_in);
+  const BalanceSeq q = balance_seq(a, room, SEQ_SMEM);
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  const float all = K::factor(a, __ldcg(w.docs));
+  float cnt[V], psum[V], coef = 0.0f;
+  int held = -1;  // the document that cnt and psum belong to
+  auto flush = [&]() {
+    if (held < 0) return;
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (psum[j] > 0.0f) atomicAdd(&w.sum[(uint64_t)held * a.E + K::expert(j)], __float2ull_rn(psum[j] * UNIT));
+  };
+#pragma unroll
+  for (int j = 0; j < V; j++) cnt[j] = psum[j] = 0.0f;
+  for (uint32_t i = 0; i < run; i++) {
+    const uint32_t t = first_t + i * K::GROUPS;
+    if (t >= a.T) break;
+    K tok = next;
+    if (i + 1 < run && t + K::GROUPS < a.T) next.load(a, t + K::GROUPS, vec_in);
+    const int s = q.doc(a, t);
+    if (s >= 0) {
+      if (s != held) {
+        flush();
+        held = s;
+        const float n = (float)__ldcg(&w.tokens[s]);
+        coef = all / n / n;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          psum[j] = 0.0f;
+          cnt[j] = K::expert(j) < a.E ? (float)__ldcg(&a.counts[(uint64_t)s * a.E + K::expert(j)]) : 0.0f;
         }
       }
+      tok.softmax(cnt, psum, coef, &w.bad[s]);
+    } else {
+      tok.scale = tok.mean = tok.fill = 0.0f;
     }
-    __syncthreads();
+    if (a.grad) tok.write(a, t, cnt, vec_out);
+  }
+  // one row of sums a warp where all its groups hold the same document
+  const int first = __shfl_sync(0xffffffffu, held, 0);
+  const bool same = __all_sync(0xffffffffu, held == first || held < 0) && first >= 0;
+  if (same) {
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+#pragma unroll
+      for (int d = L; d < 32; d <<= 1) psum[j] += __shfl_xor_sync(0xffffffffu, psum[j], d);
+      if (K::group() == 0) red[warp][K::expert(j)] = psum[j];
+    }
+  } else {
+    flush();
+  }
+  if (lane == 0) red_doc[warp] = same ? first : -1;
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < a.E; e += THREADS) {
+    float sum = 0.0f;
+    for (uint32_t i = 0; i < WARPS; i++) {
+      const int s = red_doc[i];
+      if (s >= 0) sum += red[i][e];
+      if (s >= 0 && (i + 1 == WARPS || red_doc[i + 1] != s)) {
+        atomicAdd(&w.sum[(uint64_t)s * a.E + e], __float2ull_rn(sum * UNIT));
+        sum = 0.0f;
+      }
+    }
   }
 }
 
-// Mean probabilities and the loss: a partial sum for each block, added by the last.
-__device__ __forceinline__ void balance_loss(const BalanceArgs& a, uint32_t bid, uint32_t nb) {
-  using namespace bal;
+// A document's mean probability of an expert, from its sum in units of 2^-40,
+// and the entry's part of the loss.
+__device__ __forceinline__ double balance_entry(const BalanceArgs& a, uint64_t i, unsigned long long sum, int n, bool bad,
+                                                int count) {
+  double p = n > 0 ? (double)sum * (1.0 / (double)bal::UNIT) / n : 0.0;
+  if (bad) p = __longlong_as_double(0x7ff8000000000000ll);
+  a.prob[i] = (float)p;
+  return n > 0 ? p * count * ((double)a.E / ((double)a.k * n)) : 0.0;
+}
+
+template <uint32_t WARPS>
+__device__ __forceinline__ double balance_block_sum(double v) {
   __shared__ double warp_sum[WARPS];
-  const BalanceWork w = balance_work(a);
-  auto block_sum = [&](double v) {
 #pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0;
-    for (uint32_t i = 0; i < WARPS; i++) v += warp_sum[i];
-    return v;
-  };
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+  for (uint32_t i = 0; i < WARPS; i++) v += warp_sum[i];
+  return v;
+}
+
+// Mean probabilities and the loss: a partial sum for each block, added by the last.
+__global__ void __launch_bounds__(bal::THREADS) balance_loss_kernel(const BalanceArgs a) {
+  using namespace bal;
+  pdl_wait();
+  pdl_trigger();
+  const BalanceWork w = balance_work(a);
   double sum = 0.0;
-  if (bid < a.loss_blocks) {
-    for (uint64_t i = bid * THREADS + threadIdx.x; i < (uint64_t)a.S * a.E; i += a.loss_blocks * THREADS) {
-      const uint32_t s = (uint32_t)(i / a.E);
-      const int n = __ldcg(&w.tokens[s]);
-      double p = n > 0 ? (double)__ldcg(&w.sum[i]) * (1.0 / (double)UNIT) / n : 0.0;
-      if (__ldcg(&w.bad[s])) p = __longlong_as_double(0x7ff8000000000000ll);
-      a.prob[i] = (float)p;
-      if (n > 0) sum += p * __ldcg(&a.counts[i]) * ((double)a.E / ((double)a.k * n));
-    }
-    sum = block_sum(sum);
-    if (threadIdx.x == 0) w.part[bid] = sum;
+  for (uint64_t i = (uint64_t)blockIdx.x * THREADS + threadIdx.x; i < (uint64_t)a.S * a.E; i += gridDim.x * THREADS) {
+    const uint32_t s = i >> 32 ? (uint32_t)(i / a.E) : (uint32_t)i / a.E;
+    sum += balance_entry(a, i, __ldcg(&w.sum[i]), __ldcg(&w.tokens[s]), __ldcg(&w.bad[s]) != 0, __ldcg(&a.counts[i]));
   }
-  if (balance_last(&w.ticket[1], nb)) {
-    sum = block_sum(threadIdx.x < a.loss_blocks ? __ldcg(&w.part[threadIdx.x]) : 0.0);
+  sum = balance_block_sum<WARPS>(sum);
+  if (threadIdx.x == 0) w.part[blockIdx.x] = sum;
+  if (balance_last(&w.ticket[1], gridDim.x)) {
+    sum = balance_block_sum<WARPS>(threadIdx.x < gridDim.x ? __ldcg(&w.part[threadIdx.x]) : 0.0);
     if (threadIdx.x == 0) *a.loss = (float)(sum * a.alpha / max(__ldcg(w.docs), 1));
   }
 }
 
-__global__ void __launch_bounds__(bal::THREADS) balance_clear_kernel(const BalanceArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  balance_clear(a, blockIdx.x, gridDim.x);
-}
-__global__ void __launch_bounds__(bal::THREADS) balance_count_kernel(const BalanceArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  balance_count(a, blockIdx.x, gridDim.x);
-}
+// Everything by one block: counts and sums in shared memory, the sums as two
+// words of 20 bits of 2^-40 and 2^-20 (at most 2^10 tokens: both stay below
+// 2^31), whose atomics are native.
+struct BalanceOne {
+  int seq[bal::ONE_TABLE + 1];
+  int tokens[bal::ONE_TABLE], bad[bal::ONE_TABLE];
+  int doc[bal::ONE_TOKENS];
+  int counts[bal::ONE_TABLE];
+  uint32_t hi[bal::ONE_TABLE], lo[bal::ONE_TABLE];
+};
 template <int DT, int L, int V>
-__global__ void __launch_bounds__(bal::THREADS) balance_tokens_kernel(const BalanceArgs a) {
-  pdl_trigger();
+__global__ void __launch_bounds__(bal::ONE_THREADS, 1) balance_one_kernel(const BalanceArgs a) {
+  using namespace bal;
+  using K = BalanceToken<DT, L, V>;
+  extern __shared__ __align__(16) uint8_t one_smem[];
+  BalanceOne& m = *reinterpret_cast<BalanceOne*>(one_smem);
   pdl_wait();
-  balance_tokens<DT, L, V>(a, blockIdx.x, gridDim.x);
-}
-__global__ void __launch_bounds__(bal::THREADS) balance_loss_kernel(const BalanceArgs a) {
   pdl_trigger();
-  pdl_wait();
-  balance_loss(a, blockIdx.x, gridDim.x);
-}
-
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// All phases by one cluster.
-template <int DT, int L, int V>
-__global__ void __launch_bounds__(bal::THREADS) balance_cluster_kernel(const BalanceArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  balance_clear(a, blockIdx.x, bal::CLUSTER);
-  cluster_sync();
-  balance_count(a, blockIdx.x, bal::CLUSTER);
-  cluster_sync();
-  balance_tokens<DT, L, V>(a, blockIdx.x, bal::CLUSTER);
-  cluster_sync();
-  balance_loss(a, blockIdx.x, bal::CLUSTER);
+  constexpr uint32_t STRIDE = ONE_THREADS / 32 * K::GROUPS;
+  const uint32_t first_t = threadIdx.x / L;
+  const bool vec_in = K::vec_in(a), vec_out = K::vec_out(a);
+  K next;
+  if (first_t < a.T) next.load(a, first_t, vec_in);
+  const BalanceSeq q = balance_seq(a, m.seq, ONE_TABLE + 1);
+  const uint32_t table = a.S * a.E;
+  for (uint32_t i = threadIdx.x; i < table; i += ONE_THREADS) m.counts[i] = m.hi[i] = m.lo[i] = 0;
+  for (uint32_t i = threadIdx.x; i < a.S; i += ONE_THREADS) m.tokens[i] = m.bad[i] = 0;
+  __syncthreads();
+  {
+    const int s = threadIdx.x < a.T ? q.doc(a, threadIdx.x) : -1;
+    m.doc[threadIdx.x] = s;
+    const uint32_t alike = __match_any_sync(0xffffffffu, s);  // one add for each document of a warp
+    if (s >= 0 && (threadIdx.x & 31) == __ffs(alike) - 1) atomicAdd(&m.tokens[s], __popc(alike));
+  }
+  __syncthreads();
+  for (uint32_t r = threadIdx.x; r < a.T * a.k; r += ONE_THREADS) {
+    const int d = m.doc[r / a.k], e = __ldg(&a.idx[r]);
+    if (d >= 0 && e >= 0 && e < (int)a.E) atomicAdd(&m.counts[d * a.E + e], 1);
+  }
+  int docs = 0;
+  for (uint32_t s0 = 0; s0 < a.S; s0 += ONE_THREADS)
+    docs += __syncthreads_count(s0 + threadIdx.x < a.S && m.tokens[min(s0 + threadIdx.x, a.S - 1)] > 0);
+  const float all = K::factor(a, docs);
+  for (uint32_t t = first_t; t < a.T; t += STRIDE) {
+    K tok = next;
+    if (t + STRIDE < a.T) next.load(a, t + STRIDE, vec_in);
+    const int s = m.doc[t];
+    float cnt[V], psum[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      psum[j] = 0.0f;
+      cnt[j] = s >= 0 && K::expert(j) < a.E ? (float)m.counts[s * a.E + K::expert(j)] : 0.0f;
+    }
+    if (s >= 0) {
+      const float n = (float)m.tokens[s];
+      tok.softmax(cnt, psum, all / n / n, &m.bad[s]);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const unsigned long long u = __float2ull_rn(psum[j] * UNIT);
+        if (!u) continue;
+        atomicAdd(&m.hi[s * a.E + K::expert(j)], (uint32_t)(u >> 20));
+        atomicAdd(&m.lo[s * a.E + K::expert(j)], (uint32_t)u & 0xfffffu);
+      }
+    } else {
+      tok.scale = tok.mean = tok.fill = 0.0f;
+    }
+    if (a.grad) tok.write(a, t, cnt, vec_out);
+  }
+  __syncthreads();
+  double sum = 0.0;
+  for (uint32_t i = threadIdx.x; i < table; i += ONE_THREADS) {
+    const uint32_t s = i / a.E;
+    const unsigned long long u = ((unsigned long long)m.hi[i] << 20) + m.lo[i];
+    sum += balance_entry(a, i, u, m.tokens[s], m.bad[s] != 0, m.counts[i]);
+    a.counts[i] = m.counts[i];
+  }
+  sum = balance_block_sum<ONE_THREADS / 32>(sum);
+  if (threadIdx.x == 0) *a.loss = (float)(sum * a.alpha / max(docs, 1));
 }
 
 template <int DT, int L, int V>
 static cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st) {
   using namespace bal;
   const uint64_t table = (uint64_t)a.S * a.E;
-  if ((uint64_t)a.T * std::max(a.E, 64u) <= kBalanceClusterLogits && table <= kBalanceClusterLogits / 4) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(CLUSTER);
-    cfg.blockDim = dim3(THREADS);
-    cfg.stream = st;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = CLUSTER;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, balance_cluster_kernel<DT, L, V>, a);
+  if ((uint64_t)a.T * std::max(a.E, 64u) <= kBalanceOneLogits && a.T <= ONE_TOKENS && table <= ONE_TABLE) {
+    static std::atomic<uint64_t> attr_done{0};
+    if (cudaError_t e = smem_attr_per_device(balance_one_kernel<DT, L, V>, (int)sizeof(BalanceOne), attr_done);
+        e != cudaSuccess)
+      return e;
+    return launch_pdl(balance_one_kernel<DT, L, V>, dim3(1), dim3(ONE_THREADS), sizeof(BalanceOne), st, a);
   }
-  constexpr uint32_t TILE = WARPS * (32 / L) * RUN;
   const dim3 t(THREADS);
   const uint32_t clear = (uint32_t)std::min<uint64_t>((std::max<uint64_t>(table, 2ull * a.S + 3) + THREADS - 1) / THREADS, 1024);
   cudaError_t e = launch_pdl(balance_clear_kernel, dim3(clear), t, 0, st, a);
-  const uint32_t count = std::max(1u, (a.T + COUNT_TOKENS - 1) / COUNT_TOKENS);
-  if (e == cudaSuccess) e = launch_pdl(balance_count_kernel, dim3(count), t, 0, st, a);
-  if (e == cudaSuccess && a.T) e = launch_pdl(balance_tokens_kernel<DT, L, V>, dim3((a.T + TILE - 1) / TILE), t, 0, st, a);
+  const uint32_t count = (a.T + COUNT_TOKENS - 1) / COUNT_TOKENS;
+  if (e == cudaSuccess && count) e = launch_pdl(balance_count_kernel, dim3(count), t, 0, st, a);
+  if (e == cudaSuccess && a.T) {
+    // runs as long as four blocks an SM still have one
+    const uint32_t at_once = WARPS * (32 / L), wave = (uint32_t)num_sms() * 4 * at_once;
+    const uint32_t run = std::min(MAX_RUN, (a.T + wave - 1) / wave), tile = at_once * run;
+    e = launch_pdl(balance_tokens_kernel<DT, L, V>, dim3((a.T + tile - 1) / tile), t, 0, st, a, run);
+  }
   if (e == cudaSuccess) e = launch_pdl(balance_loss_kernel, dim3(a.loss_blocks), t, 0, st, a);
   return e;
 }
 
 template <int DT>
 static cudaError_t launch_balance_experts(const BalanceArgs& a, cudaStream_t st) {
-  if (a.E <= 128) return launch_balance<DT, 8, 16>(a, st);
-  if (a.E <= 256) return launch_balance<DT, 16, 16>(a, st);
-  if (a.E <= 512) return launch_balance<DT, 32, 16>(a, st);
+  if (a.E <= 64) return launch_balance<DT, 8, 8>(a, st);
+  if (a.E <= 128) return launch_balance<DT, 16, 8>(a, st);
+  if (a.E <= 256) return launch_balance<DT, 32, 8>(a, st);
   return launch_balance<DT, 32, 32>(a, st);
 }
 

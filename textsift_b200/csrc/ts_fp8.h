@@ -91,8 +91,8 @@ struct BalanceArgs {
   uint32_t loss_blocks = 1;  // set by the launcher
 };
 constexpr uint32_t kBalanceMaxExperts = 1024, kBalanceMaxK = 64, kBalanceMaxTokens = 1u << 23;
-// Calls of at most this many logits run as one cluster.
-constexpr uint64_t kBalanceClusterLogits = 1u << 17;
+// Calls of at most this many logits may run as one block.
+constexpr uint64_t kBalanceOneLogits = 1u << 16;
 size_t balance_work_bytes(uint32_t S, uint32_t E);
 cudaError_t launch_router_balance(BalanceArgs a, cudaStream_t st);
 
