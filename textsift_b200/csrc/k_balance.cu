@@ -24,6 +24,7 @@ namespace ts {
 namespace bal {
 constexpr uint32_t THREADS = 256, WARPS = 8;
 constexpr uint32_t COUNT_TOKENS = 256;  // tokens of a counting tile
+constexpr uint32_t COUNT_AHEAD = 4;     // of its routes, those a thread loads at once
 constexpr uint32_t MAX_RUN = 16;        // most tokens a lane group takes in a row
 constexpr uint32_t SEQ_SMEM = 1024;     // document offsets that a block keeps in shared memory
 constexpr uint32_t MAX_LOSS_BLOCKS = 256;
@@ -37,13 +38,12 @@ static uint32_t balance_loss_blocks(uint32_t S, uint32_t E) {
 }
 
 // Work area: sums u64 [S][E], partial losses f64 [blocks], tokens i32 [S],
-// poisoned i32 [S], then documents with tokens and two tickets.
+// poisoned i32 [S], then a ticket.
 struct BalanceWork {
   unsigned long long* sum;
   double* part;
   int* tokens;
   int* bad;
-  int* docs;
   unsigned* ticket;
 };
 __device__ __forceinline__ BalanceWork balance_work(const BalanceArgs& a) {
@@ -52,21 +52,21 @@ __device__ __forceinline__ BalanceWork balance_work(const BalanceArgs& a) {
   w.part = reinterpret_cast<double*>(w.sum + (uint64_t)a.S * a.E);
   w.tokens = reinterpret_cast<int*>(w.part + a.loss_blocks);
   w.bad = w.tokens + a.S;
-  w.docs = w.bad + a.S;
-  w.ticket = reinterpret_cast<unsigned*>(w.docs + 1);
+  w.ticket = reinterpret_cast<unsigned*>(w.bad + a.S);
   return w;
 }
 size_t balance_work_bytes(uint32_t S, uint32_t E) {
-  return (size_t)S * E * 8 + balance_loss_blocks(S, E) * 8 + (size_t)S * 8 + 12;
+  return (size_t)S * E * 8 + balance_loss_blocks(S, E) * 8 + (size_t)S * 8 + 4;
 }
+
+__device__ __forceinline__ bool balance_token(const BalanceArgs& a, uint32_t t) { return !a.mask || __ldg(&a.mask[t]); }
 
 // Document offsets as a block sees them: in shared memory when there are few.
 struct BalanceSeq {
   const int* at;  // null: one document of all tokens
   uint32_t S;
-  // The document of token t, or -1: padding, or outside [seq[0], seq[S]).
-  __device__ __forceinline__ int doc(const BalanceArgs& a, uint32_t t) const {
-    if (a.mask && !a.mask[t]) return -1;
+  // The document of token t, or -1 outside [seq[0], seq[S]).
+  __device__ __forceinline__ int doc(uint32_t t) const {
     if (!at) return 0;
     if ((int)t < at[0] || (int)t >= at[S]) return -1;
     uint32_t lo = 0, hi = S;  // at[lo] <= t < at[hi]
@@ -77,6 +77,7 @@ struct BalanceSeq {
     }
     return (int)lo;
   }
+  __device__ __forceinline__ uint32_t end(int s) const { return at ? (uint32_t)max(at[s + 1], 0) : 0xffffffffu; }
 };
 // Copies the offsets into `room` where they fit; the caller synchronizes.
 __device__ __forceinline__ BalanceSeq balance_seq(const BalanceArgs& a, int* room, uint32_t size) {
@@ -86,6 +87,14 @@ __device__ __forceinline__ BalanceSeq balance_seq(const BalanceArgs& a, int* roo
     q.at = room;
   }
   return q;
+}
+
+// Documents with tokens, by the whole block.
+__device__ __forceinline__ int balance_docs(const BalanceArgs& a, const int* tokens) {
+  int docs = 0;
+  for (uint32_t s0 = 0; s0 < a.S; s0 += blockDim.x)
+    docs += __syncthreads_count(s0 + threadIdx.x < a.S && __ldcg(&tokens[min(s0 + threadIdx.x, a.S - 1)]) > 0);
+  return docs;
 }
 
 // True in every thread of the block that is the last of nb to come here; what
@@ -112,12 +121,11 @@ __global__ void __launch_bounds__(bal::THREADS) balance_clear_kernel(const Balan
     w.sum[i] = 0;
     a.counts[i] = 0;
   }
-  for (uint64_t i = (uint64_t)blockIdx.x * bal::THREADS + threadIdx.x; i < 2ull * a.S + 3; i += step) w.tokens[i] = 0;
+  for (uint64_t i = (uint64_t)blockIdx.x * bal::THREADS + threadIdx.x; i < 2ull * a.S + 1; i += step) w.tokens[i] = 0;
 }
 
 // Counts of a tile of 256 tokens: through shared memory where the tile lies in
-// one document, straight to the document's row where it does not.  The last
-// block counts the documents that have tokens.
+// one document, straight to the document's row where it does not.
 __global__ void __launch_bounds__(bal::THREADS) balance_count_kernel(const BalanceArgs a) {
   using namespace bal;
   __shared__ int hist[kBalanceMaxExperts];
@@ -125,10 +133,18 @@ __global__ void __launch_bounds__(bal::THREADS) balance_count_kernel(const Balan
   __shared__ int room[SEQ_SMEM];
   __shared__ int top[WARPS];
   const BalanceWork w = balance_work(a);
+  const uint32_t t0 = blockIdx.x * COUNT_TOKENS, t = t0 + threadIdx.x, n = min(COUNT_TOKENS, a.T - t0);
+  // every input is on its way before the first is waited for
+  int route[COUNT_AHEAD];
+#pragma unroll
+  for (uint32_t j = 0; j < COUNT_AHEAD; j++) {
+    const uint32_t r = threadIdx.x + j * THREADS;
+    route[j] = r < n * a.k ? __ldg(&a.idx[(uint64_t)t0 * a.k + r]) : -1;
+  }
+  const bool token = t < a.T && balance_token(a, t);
   const BalanceSeq q = balance_seq(a, room, SEQ_SMEM);
   __syncthreads();
-  const uint32_t t0 = blockIdx.x * COUNT_TOKENS, t = t0 + threadIdx.x, n = min(COUNT_TOKENS, a.T - t0);
-  const int s = t < a.T ? q.doc(a, t) : -1;
+  const int s = token ? q.doc(t) : -1;
   doc[threadIdx.x] = s;
   for (uint32_t e = threadIdx.x; e < a.E; e += THREADS) hist[e] = 0;
   // the tile's one document: the largest of all, equal to every one that is not padding
@@ -148,22 +164,21 @@ __global__ void __launch_bounds__(bal::THREADS) balance_count_kernel(const Balan
     } else if (s >= 0) {
       atomicAdd(&w.tokens[s], 1);
     }
-    for (uint32_t r = threadIdx.x; r < n * a.k; r += THREADS) {
-      const int d = doc[r / a.k], e = __ldg(&a.idx[(uint64_t)t0 * a.k + r]);
-      if (d < 0 || e < 0 || e >= (int)a.E) continue;
+    auto count = [&](uint32_t r, int e) {
+      if (e < 0 || e >= (int)a.E) return;
+      const int d = doc[r / a.k];
+      if (d < 0) return;
       if (single) atomicAdd(&hist[e], 1);
       else atomicAdd(&a.counts[(uint64_t)d * a.E + e], 1);
-    }
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < COUNT_AHEAD; j++) count(threadIdx.x + j * THREADS, route[j]);
+    for (uint32_t r = threadIdx.x + COUNT_AHEAD * THREADS; r < n * a.k; r += THREADS)
+      count(r, __ldg(&a.idx[(uint64_t)t0 * a.k + r]));
     __syncthreads();
     if (single)
       for (uint32_t e = threadIdx.x; e < a.E; e += THREADS)
         if (hist[e]) atomicAdd(&a.counts[(uint64_t)one * a.E + e], hist[e]);
-  }
-  if (balance_last(&w.ticket[0], gridDim.x)) {
-    int used = 0;
-    for (uint32_t s0 = 0; s0 < a.S; s0 += THREADS)
-      used += __syncthreads_count(s0 + threadIdx.x < a.S && __ldcg(&w.tokens[min(s0 + threadIdx.x, a.S - 1)]) > 0);
-    if (threadIdx.x == 0) *w.docs = used;
   }
 }
 
@@ -175,8 +190,11 @@ struct BalanceToken {
   using T = typename D::T;
   static constexpr int PER = 16 / (int)sizeof(T), GROUPS = 32 / L;
   static_assert(V % PER == 0, "whole pieces");
-  float z[V];           // logits, then probabilities
-  float scale, mean, fill;  // gradient: scale * p * (count - mean), or fill where scale is 0
+  float z[V];  // logits, then e^(logit - largest)
+  // the gradient is z * (count * slope + base): slope = coef / sum and base =
+  // -mean count * slope; both 0 for padding and for a row with nothing open,
+  // NaN for one that holds a NaN or +inf
+  float slope, base;
 
   static __device__ __forceinline__ uint32_t lane() { return threadIdx.x % L; }
   static __device__ __forceinline__ uint32_t group() { return (threadIdx.x & 31) / L; }
@@ -201,11 +219,17 @@ struct BalanceToken {
       }
     }
   }
-  // Probabilities and the gradient's terms of a token of document s; adds the
-  // probabilities to psum.
+  __device__ __forceinline__ void nothing() {
+    slope = base = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; j++) z[j] = 0.0f;
+  }
+  // The exponentials and the gradient's terms of a token; adds its
+  // probabilities to psum.  e^x is 2^(x log2 e) on the special-function unit,
+  // x <= 0 the difference to the largest logit: off by 2^-22 and by 2^-24 |x|
+  // log2 e of the value, which is e^x of the largest.
   __device__ __forceinline__ void softmax(const float (&cnt)[V], float (&psum)[V], float coef, int* bad) {
     const float inf = __int_as_float(0x7f800000);
-    scale = mean = fill = 0.0f;
     float m = -inf, sum = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; j++) m = fmaxf(m, z[j]);
@@ -219,7 +243,7 @@ struct BalanceToken {
     } else {
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        z[j] = expf(z[j] - m);
+        z[j] = ex2_approx((z[j] - m) * 1.4426950408889634f);
         sum += z[j];
         dot = fmaf(z[j], cnt[j], dot);
       }
@@ -230,17 +254,17 @@ struct BalanceToken {
       }
       odd = !(sum == sum);  // a NaN among finite logits
     }
-    if (odd) {
-      if (lane() == 0) *bad = 1;
-      fill = __int_as_float(0x7fc00000);
-    } else if (sum > 0.0f) {
+    if (sum > 0.0f) {
       const float inv = 1.0f / sum;
-      mean = dot * inv;
-      scale = coef;
+      slope = coef * inv;
+      base = -(dot * inv) * slope;
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        z[j] *= inv;
-        psum[j] += z[j];
+      for (int j = 0; j < V; j++) psum[j] = fmaf(z[j], inv, psum[j]);
+    } else {
+      nothing();
+      if (odd) {
+        slope = base = __int_as_float(0x7fc00000);
+        if (lane() == 0) *bad = 1;
       }
     }
   }
@@ -252,7 +276,7 @@ struct BalanceToken {
       uint4 raw;
       T* out = reinterpret_cast<T*>(&raw);
 #pragma unroll
-      for (int i = 0; i < PER; i++) out[i] = D::down(scale != 0.0f ? scale * z[j + i] * (cnt[j + i] - mean) : fill);
+      for (int i = 0; i < PER; i++) out[i] = D::down(z[j + i] * fmaf(cnt[j + i], slope, base));
       if (vec && e + PER <= a.E) {
         *reinterpret_cast<uint4*>(g + e) = raw;
       } else {
@@ -279,7 +303,7 @@ struct BalanceToken {
 // its counts and the sums of its probabilities stay in registers until the
 // document ends.
 template <int DT, int L, int V>
-__global__ void __launch_bounds__(bal::THREADS) balance_tokens_kernel(const BalanceArgs a, uint32_t run) {
+__global__ void __launch_bounds__(bal::THREADS, V <= 8 ? 4 : 1) balance_tokens_kernel(const BalanceArgs a, uint32_t run) {
   using namespace bal;
   using K = BalanceToken<DT, L, V>;
   __shared__ float red[WARPS][L * V];
@@ -290,14 +314,20 @@ __global__ void __launch_bounds__(bal::THREADS) balance_tokens_kernel(const Bala
   const bool vec_in = K::vec_in(a), vec_out = K::vec_out(a);
   const uint32_t first_t = (blockIdx.x * WARPS + warp) * run * K::GROUPS + K::group();
   K next;
-  if (first_t < a.T) next.load(a, first_t, vec_in);
+  bool next_token = false;
+  if (first_t < a.T) {
+    next.load(a, first_t, vec_in);
+    next_token = balance_token(a, first_t);
+  }
   const BalanceSeq q = balance_seq(a, room, SEQ_SMEM);
   __syncthreads();
   pdl_wait();
   pdl_trigger();
-  const float all = K::factor(a, __ldcg(w.docs));
+  const float all = K::factor(a, balance_docs(a, w.tokens));
   float cnt[V], psum[V], coef = 0.0f;
-  int held = -1;  // the document that cnt and psum belong to
+  int held = -1;      // the document that cnt and psum belong to
+  int now = -1;       // the document of the group's tokens
+  uint32_t end = 0;   // where that is to be looked up again
   auto flush = [&]() {
     if (held < 0) return;
 #pragma unroll
@@ -310,9 +340,16 @@ __global__ void __launch_bounds__(bal::THREADS) balance_tokens_kernel(const Bala
     const uint32_t t = first_t + i * K::GROUPS;
     if (t >= a.T) break;
     K tok = next;
-    if (i + 1 < run && t + K::GROUPS < a.T) next.load(a, t + K::GROUPS, vec_in);
-    const int s = q.doc(a, t);
+    const int s = next_token ? (t >= end ? q.doc(t) : now) : -1;
+    if (i + 1 < run && t + K::GROUPS < a.T) {
+      next.load(a, t + K::GROUPS, vec_in);
+      next_token = balance_token(a, t + K::GROUPS);
+    }
     if (s >= 0) {
+      if (s != now) {
+        now = s;
+        end = q.end(s);
+      }
       if (s != held) {
         flush();
         held = s;
@@ -326,7 +363,7 @@ __global__ void __launch_bounds__(bal::THREADS) balance_tokens_kernel(const Bala
       }
       tok.softmax(cnt, psum, coef, &w.bad[s]);
     } else {
-      tok.scale = tok.mean = tok.fill = 0.0f;
+      tok.nothing();
     }
     if (a.grad) tok.write(a, t, cnt, vec_out);
   }
@@ -394,9 +431,10 @@ __global__ void __launch_bounds__(bal::THREADS) balance_loss_kernel(const Balanc
   }
   sum = balance_block_sum<WARPS>(sum);
   if (threadIdx.x == 0) w.part[blockIdx.x] = sum;
-  if (balance_last(&w.ticket[1], gridDim.x)) {
+  if (balance_last(w.ticket, gridDim.x)) {
     sum = balance_block_sum<WARPS>(threadIdx.x < gridDim.x ? __ldcg(&w.part[threadIdx.x]) : 0.0);
-    if (threadIdx.x == 0) *a.loss = (float)(sum * a.alpha / max(__ldcg(w.docs), 1));
+    const int docs = balance_docs(a, w.tokens);
+    if (threadIdx.x == 0) *a.loss = (float)(sum * a.alpha / max(docs, 1));
   }
 }
 
@@ -429,7 +467,7 @@ __global__ void __launch_bounds__(bal::ONE_THREADS, 1) balance_one_kernel(const 
   for (uint32_t i = threadIdx.x; i < a.S; i += ONE_THREADS) m.tokens[i] = m.bad[i] = 0;
   __syncthreads();
   {
-    const int s = threadIdx.x < a.T ? q.doc(a, threadIdx.x) : -1;
+    const int s = threadIdx.x < a.T && balance_token(a, threadIdx.x) ? q.doc(threadIdx.x) : -1;
     m.doc[threadIdx.x] = s;
     const uint32_t alike = __match_any_sync(0xffffffffu, s);  // one add for each document of a warp
     if (s >= 0 && (threadIdx.x & 31) == __ffs(alike) - 1) atomicAdd(&m.tokens[s], __popc(alike));
@@ -464,7 +502,7 @@ __global__ void __launch_bounds__(bal::ONE_THREADS, 1) balance_one_kernel(const 
         atomicAdd(&m.lo[s * a.E + K::expert(j)], (uint32_t)u & 0xfffffu);
       }
     } else {
-      tok.scale = tok.mean = tok.fill = 0.0f;
+      tok.nothing();
     }
     if (a.grad) tok.write(a, t, cnt, vec_out);
   }
@@ -492,7 +530,7 @@ static cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st) {
     return launch_pdl(balance_one_kernel<DT, L, V>, dim3(1), dim3(ONE_THREADS), sizeof(BalanceOne), st, a);
   }
   const dim3 t(THREADS);
-  const uint32_t clear = (uint32_t)std::min<uint64_t>((std::max<uint64_t>(table, 2ull * a.S + 3) + THREADS - 1) / THREADS, 1024);
+  const uint32_t clear = (uint32_t)std::min<uint64_t>((std::max<uint64_t>(table, 2ull * a.S + 1) + THREADS - 1) / THREADS, 1024);
   cudaError_t e = launch_pdl(balance_clear_kernel, dim3(clear), t, 0, st, a);
   const uint32_t count = (a.T + COUNT_TOKENS - 1) / COUNT_TOKENS;
   if (e == cudaSuccess && count) e = launch_pdl(balance_count_kernel, dim3(count), t, 0, st, a);

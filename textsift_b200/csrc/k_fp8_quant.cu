@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(256, 8) fp8_quant_rows_kernel(const Fp8QuantAr
 // leave as one line.  Four words after every 16 rows put the eight lanes'
 // rows into different banks.
 template <int DT>
-__global__ void __launch_bounds__(256) fp8_quant_cols_kernel(const Fp8QuantArgs a, uint32_t vec, uint32_t col_tiles) {
+__global__ void __launch_bounds__(256, 6) fp8_quant_cols_kernel(const Fp8QuantArgs a, uint32_t vec, uint32_t col_tiles) {
   using D = Fp8Type<DT>;
   using T = typename D::T;
   constexpr uint32_t COLS = 128 / sizeof(T), W = sizeof(T) == 2 ? 2 : 1;  // columns a lane takes
@@ -61,23 +61,20 @@ __global__ void __launch_bounds__(256) fp8_quant_cols_kernel(const Fp8QuantArgs 
   __syncthreads();
   const uint32_t col = threadIdx.x / 8 * W, g = threadIdx.x & 7;
   const uint8_t* src = tile + g * GROUP + col * sizeof(T);
-  Fp8Piece<DT> p[W];
+  uint32_t raw[16];  // of both columns
 #pragma unroll
-  for (uint32_t j = 0; j < 16; j++) {
-    T t[W];
-    if constexpr (W == 2) *reinterpret_cast<uint32_t*>(t) = *reinterpret_cast<const uint32_t*>(src + j * 128);
-    else t[0] = *reinterpret_cast<const T*>(src + j * 128);
-#pragma unroll
-    for (uint32_t w = 0; w < W; w++) p[w].v[j] = D::up(t[w]);
-  }
+  for (uint32_t j = 0; j < 16; j++) raw[j] = *reinterpret_cast<const uint32_t*>(src + j * 128);
   const uint32_t row0 = b * kFp8Block + g * 16;
 #pragma unroll
   for (uint32_t w = 0; w < W; w++) {
-    const float s = fp8_scale(p[w].block_max());
+    Fp8Piece<DT> p;
+#pragma unroll
+    for (uint32_t j = 0; j < 16; j++) p.v[j] = D::up(reinterpret_cast<const T*>(&raw[j])[w]);
+    const float s = fp8_scale(p.block_max());
     const uint64_t c = c0 + col + w;
     if (c >= a.cols) continue;
     if (g == 0) a.scales[b * a.lds + c] = s;
-    if (row0 < a.rows) *reinterpret_cast<uint4*>(a.codes + c * a.ldc + row0) = p[w].codes(fp8_inverse(s));
+    if (row0 < a.rows) *reinterpret_cast<uint4*>(a.codes + c * a.ldc + row0) = p.codes(fp8_inverse(s));
   }
 }
 
