@@ -47,10 +47,13 @@ template <int BN>
 struct Cfg {
   static constexpr uint32_t W_BYTES = BN * kFp8Block;
   static constexpr uint32_t STAGE = A_BYTES + W_BYTES;
-  static constexpr uint32_t S = 196608 / STAGE;       // 192 KB of stages
+  static constexpr uint32_t S = BN == 256 ? 3 : BN == 128 ? 4 : 6;
   static constexpr uint32_t NB = TMEM_COLS / BN;      // TMEM buffers
   static constexpr uint32_t PART = BN / 4;            // columns a warp owns
-  static constexpr uint32_t OFF_BAR = S * STAGE;
+  // a warp's rows on their way out: 32 of up to 128 bytes
+  static constexpr uint32_t OUT_BYTES = 32 * (PART * 4 < 128 ? PART * 4 : 128);
+  static constexpr uint32_t OFF_OUT = S * STAGE;
+  static constexpr uint32_t OFF_BAR = OFF_OUT + DRAIN_WARPS * OUT_BYTES;
   static constexpr uint32_t NUM_BARS = 2 * S + 2 * NB + 1;
   static constexpr uint32_t OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr uint32_t OFF_SEG = OFF_MISC + 16;  // tile prefix of the segments, then their first rows
@@ -110,12 +113,23 @@ __device__ __forceinline__ void fp8_tmem_ld(uint32_t addr, uint32_t (&r)[N]) {
   else tmem_ld_32x32b_x16(addr, r);
 }
 
-// 32 bytes at a 32-byte aligned address.
-__device__ __forceinline__ void st_global_32(void* p, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* smem_src, int32_t c0, int32_t c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(c0), "r"(c1), "r"(smem_u32(smem_src))
                : "memory");
 }
+// The same, added to what is there (f32).
+__device__ __forceinline__ void tma_add_2d(const void* tmap, const void* smem_src, int32_t c0, int32_t c1) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(c0), "r"(c1), "r"(smem_u32(smem_src))
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// The thread's bulk stores have read their shared memory.
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 template <int OT>
 __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
@@ -128,27 +142,54 @@ __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
   }
 }
 
-// The PART columns from n of row m: acc + bias (+ what out holds).
-template <int OT, int PART>
-__device__ __forceinline__ void fp8_write_row(const Fp8MmArgs& a, uint32_t e, uint32_t m, uint32_t n,
-                                              const uint64_t (&acc)[PART / 2]) {
-  using D = Fp8Type<OT>;
-  auto* o = reinterpret_cast<typename D::T*>(a.out) + m * a.ldo + n;
-  const __half* bias = a.bias ? reinterpret_cast<const __half*>(a.bias) + (uint64_t)e * a.N + n : nullptr;
-  const bool whole = n + PART <= a.N && !(reinterpret_cast<uintptr_t>(o) & 31u) && !a.accumulate;
-  if (whole) {
-    constexpr int PER = 32 / (int)sizeof(typename D::T);  // values of a 32-byte store
+// 16 bytes of bias: the 8 columns from n.
+__device__ __forceinline__ void fp8_bias8(const __half* bias, uint32_t n, uint32_t N, float (&b)[8]) {
+  if (n + 8 <= N && !(reinterpret_cast<uintptr_t>(bias + n) & 15u)) {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(bias + n));
+    const __half* h = reinterpret_cast<const __half*>(&raw);
 #pragma unroll
-    for (int j = 0; j < PART; j += PER) {
+    for (int i = 0; i < 8; i++) b[i] = __half2float(h[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) b[i] = n + i < N ? __half2float(bias[n + i]) : 0.0f;
+  }
+}
+
+// Writes a warp's 32 rows (from row, those below row_end) x PART columns (from
+// n), thread = row: acc + bias (+ what out holds).  The rows go through the
+// warp's shared memory, 16-byte pieces swizzled as a tensor map of that row
+// size has them, and leave by one TMA store where all 32 rows are this tile's
+// (tma: out can be mapped), else row by row, consecutive lanes on consecutive
+// columns.
+template <int OT, int PART>
+__device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap* tmap_o, bool tma, uint8_t* stage,
+                                          uint32_t e, uint32_t row, uint32_t row_end, uint32_t n,
+                                          const uint64_t (&acc)[PART / 2]) {
+  using D = Fp8Type<OT>;
+  using T = typename D::T;
+  constexpr uint32_t RB = PART * sizeof(T) < 128 ? PART * sizeof(T) : 128;  // bytes of a staged row
+  constexpr uint32_t COLS = RB / sizeof(T), PER = 16 / sizeof(T);
+  const uint32_t lane = threadIdx.x & 31;
+  auto piece = [&](uint32_t r, uint32_t c) {  // piece c of staged row r
+    return stage + r * RB + ((c ^ ((r * RB / 128) % (RB / 16))) * 16);
+  };
+  const bool whole = tma && row + 32 <= row_end;
+#pragma unroll
+  for (uint32_t c0 = 0; c0 < PART; c0 += COLS) {
+    if (n + c0 >= a.N) break;
+    if (lane == 0) bulk_wait_read();
+    __syncwarp();
+#pragma unroll
+    for (uint32_t c = 0; c < COLS; c += 8) {
+      float b[8] = {};
+      if (a.bias) fp8_bias8(reinterpret_cast<const __half*>(a.bias) + (uint64_t)e * a.N, n + c0 + c, a.N, b);
       uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < PER; i += 2) {
+      for (uint32_t i = 0; i < 8; i += 2) {
         float x0, x1;
-        f2unpack(acc[(j + i) / 2], x0, x1);
-        if (bias) {
-          x0 += __half2float(bias[j + i]);
-          x1 += __half2float(bias[j + i + 1]);
-        }
+        f2unpack(acc[(c0 + c + i) / 2], x0, x1);
+        x0 += b[i];
+        x1 += b[i + 1];
         if constexpr (OT == TS_DTYPE_F32) {
           w[i] = __float_as_uint(x0);
           w[i + 1] = __float_as_uint(x1);
@@ -156,20 +197,28 @@ __device__ __forceinline__ void fp8_write_row(const Fp8MmArgs& a, uint32_t e, ui
           w[i / 2] = fp8_out2<OT>(x0, x1);
         }
       }
-      st_global_32(o + j, w);
+      *reinterpret_cast<uint4*>(piece(lane, c / PER)) = make_uint4(w[0], w[1], w[2], w[3]);
+      if constexpr (OT == TS_DTYPE_F32) *reinterpret_cast<uint4*>(piece(lane, c / PER + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
     }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < PART; j += 2) {
-    float x[2];
-    f2unpack(acc[j / 2], x[0], x[1]);
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      if (n + j + i >= a.N) continue;
-      float v = x[i] + (bias ? __half2float(bias[j + i]) : 0.0f);
-      if (OT == TS_DTYPE_F32 && a.accumulate) v += D::up(o[j + i]);
-      o[j + i] = D::down(v);
+    if (whole) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (OT == TS_DTYPE_F32 && a.accumulate) tma_add_2d(tmap_o, stage, (int32_t)(n + c0), (int32_t)row);
+        else tma_store_2d(tmap_o, stage, (int32_t)(n + c0), (int32_t)row);
+        bulk_commit();
+      }
+    } else {
+      __syncwarp();
+      for (uint32_t r = 0; r < 32 && row + r < row_end; r++) {
+        T* o = reinterpret_cast<T*>(a.out) + (uint64_t)(row + r) * a.ldo + n + c0;
+        for (uint32_t c = lane; c < COLS && n + c0 + c < a.N; c += 32) {
+          const T v = reinterpret_cast<const T*>(piece(r, c / PER))[c % PER];
+          if (OT == TS_DTYPE_F32 && a.accumulate) o[c] = D::down(D::up(v) + D::up(o[c]));
+          else o[c] = v;
+        }
+      }
+      __syncwarp();
     }
   }
 }
@@ -177,7 +226,7 @@ __device__ __forceinline__ void fp8_write_row(const Fp8MmArgs& a, uint32_t e, ui
 template <int BN, int WB, int OT>
 __global__ void __launch_bounds__(f8::THREADS, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
-                    const Fp8MmArgs args, uint32_t n_tiles) {
+                    const __grid_constant__ CUtensorMap tmap_o, const Fp8MmArgs args, uint32_t n_tiles, uint32_t tma_out) {
   using namespace f8;
   using C = Cfg<BN>;
   extern __shared__ uint8_t smem_dyn[];
@@ -302,6 +351,7 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
     const uint32_t q = (uint32_t)(warp & 3), p = (uint32_t)(warp - 2) >> 2;
     const uint32_t taddr = tmem_base + ((q * 32u) << 16) + p * PART;
     const uint32_t nb = fp8_blocks(args.N);
+    uint8_t* stage = smem + C::OFF_OUT + (warp - 2) * C::OUT_BYTES;
     // scales of row m and of column block (or columns) n, chunk c
     float* ring = reinterpret_cast<float*>(smem + C::OFF_WS) + (warp - 2) * PART;
     auto a_scale = [&](uint32_t m, uint32_t c) { return args.as[c * args.ldas + min(m, args.M - 1)]; };
@@ -386,8 +436,9 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
         ti = fp8_tile(args, t + gridDim.x, m_tiles, n_tiles, BN, pre, first);
         ahead(ti);
       }
-      if (m < done.row_end && done.n0 + p * PART < args.N) fp8_write_row<OT, PART>(args, done.e, m, done.n0 + p * PART, acc);
+      fp8_write<OT, PART>(args, &tmap_o, tma_out, stage, done.e, done.row0 + q * 32u, done.row_end, done.n0 + p * PART, acc);
     }
+    if (lane == 0) bulk_wait();
   }
   tc_fence_before();
   __syncthreads();
@@ -406,7 +457,12 @@ static cudaError_t launch_gemm(const CUtensorMap& ta, const CUtensorMap& tw, con
   if (cudaError_t e = smem_attr_per_device(fp8_gemm_kernel<BN, WB, OT>, (int)smem, attr_done); e != cudaSuccess) return e;
   const uint32_t n_tiles = (a.N + BN - 1) / BN;
   const uint32_t grid = (uint32_t)std::min<uint64_t>(m_tiles * n_tiles, (uint64_t)num_sms());
-  return launch_pdl(fp8_gemm_kernel<BN, WB, OT>, dim3(grid), dim3(f8::THREADS), smem, st, ta, tw, a, n_tiles);
+  // out as 16-byte pieces of rows that can be mapped: the tensor map's box is a
+  // warp's 32 rows of up to 128 bytes
+  constexpr uint32_t size = sizeof(typename Fp8Type<OT>::T), bytes = std::min<uint32_t>(C::PART * size, 128);
+  CUtensorMap to = ta;
+  const uint32_t tma_out = make_out_tmap(&to, a.out, OT, a.M, a.N, a.ldo, bytes / size, 32) ? 1 : 0;
+  return launch_pdl(fp8_gemm_kernel<BN, WB, OT>, dim3(grid), dim3(f8::THREADS), smem, st, ta, tw, to, a, n_tiles, tma_out);
 }
 
 template <int BN, int WB>
@@ -420,13 +476,16 @@ static cudaError_t launch_gemm_out(const CUtensorMap& ta, const CUtensorMap& tw,
 // K = 0: bias or zero (+ what out holds) on the rows that a segment covers.
 template <int OT>
 __global__ void __launch_bounds__(256) fp8_empty_sum_kernel(const Fp8MmArgs a) {
+  using D = Fp8Type<OT>;
   for (uint32_t e = 0; e < a.E; e++) {
     const int lo = a.seg ? min(max(a.seg[e], 0), (int)a.M) : 0;
     const int hi = a.seg ? min(max(a.seg[e + 1], 0), (int)a.M) : (int)a.M;
     for (int m = lo + (int)blockIdx.x; m < hi; m += gridDim.x)
-      for (uint32_t n = threadIdx.x * 16; n < a.N; n += 256 * 16) {
-        const uint64_t acc[8] = {};
-        fp8_write_row<OT, 16>(a, e, (uint32_t)m, n, acc);
+      for (uint32_t n = threadIdx.x; n < a.N; n += 256) {
+        auto* o = reinterpret_cast<typename D::T*>(a.out) + (uint64_t)m * a.ldo + n;
+        float v = a.bias ? __half2float(reinterpret_cast<const __half*>(a.bias)[(uint64_t)e * a.N + n]) : 0.0f;
+        if (a.accumulate) v += D::up(*o);
+        *o = D::down(v);
       }
   }
 }

@@ -27,6 +27,7 @@
 // Sharing each dequantised B tile between two 128-row accumulators halves the
 // dequantisation work per flop, which bounds this kernel's tensor-core rate.
 // All waits are bounded (ts_common.cuh) and set the device error flag.
+#include "textsift_cuda.h"
 #include "ts_common.cuh"
 #include "ts_kernels.h"
 
@@ -834,6 +835,28 @@ bool make_codes_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
+}
+
+bool make_out_tmap(CUtensorMap* map, const void* base, int dtype, uint64_t rows, uint64_t cols, uint64_t ld,
+                   uint32_t box_cols, uint32_t box_rows) {
+  const uint64_t size = dtype == TS_DTYPE_F32 ? 4 : 2, bytes = box_cols * size;
+  PFN_tmapEncodeTiled enc = get_encode_fn();
+  // a store that ends inside a 16-byte piece writes the rest of the piece too
+  if (!enc || (reinterpret_cast<uintptr_t>(base) & 15u) || (ld * size & 15u) || (cols * size & 15u) ||
+      ld * size >= 1ull << 40 || ld < cols)
+    return false;
+  cuuint64_t gdim[2] = {cols, rows};
+  cuuint64_t gstride[1] = {ld * size};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == TS_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == TS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapSwizzle swizzle = bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                   : CU_TENSOR_MAP_SWIZZLE_32B;
+  return enc(map, type, 2, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // SM count of the current device (persistent grid size), cached per device

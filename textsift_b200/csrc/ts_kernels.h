@@ -93,6 +93,12 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, uint64_t cols, uint64_t ro
 // The same for rows of K 8-bit codes, `ld` bytes apart: boxes of 128 bytes x
 // box_rows, zeros past the end of a row.
 bool make_codes_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t ld, uint32_t box_rows);
+// A 2-D map of an output [rows, cols] (TS_DTYPE_F16, BF16 or F32, ld elements
+// between rows) for TMA stores of box_rows rows of 32, 64 or 128 bytes, with
+// the swizzle of that size; false where its rows do not start and end at
+// multiples of 16 bytes.
+bool make_out_tmap(CUtensorMap* map, const void* base, int dtype, uint64_t rows, uint64_t cols, uint64_t ld,
+                   uint32_t box_cols, uint32_t box_rows);
 // Streaming multiprocessors of the current device.
 int num_sms();
 
