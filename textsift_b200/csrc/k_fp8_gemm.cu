@@ -7,22 +7,30 @@
 // the sum over blocks is taken in registers: every chunk of 128 k has a TMEM
 // buffer of its own, out of a ring, and 16 warps add it, times its scale, to
 // accumulators that stay in registers for the whole tile (64 x f32 a thread
-// at the widest).  Tiles are 128 rows of a by BN rows of w; thread = one row
-// of a, so as is one value a thread and chunk, and ws one value a warp.
+// at the widest).  Thread = one row of a, so as is one value a thread and
+// chunk, and ws one value a warp.
+//
+// Large products run on CTA pairs (cta_group::2, CG = 2): 256 rows of a by 256
+// rows of w, each CTA holding its half of both in shared memory and 128 of the
+// rows in its TMEM, so a chunk costs 32 KB of copies a CTA instead of 48; the
+// others on single CTAs with 128 rows of a by 128 or 64 of w.
 //
 // Persistent, warp-specialized, one CTA per SM:
 //   warp 0       TMA producer: per chunk a box of 128 rows x 128 bytes of a
-//                and up to BN / 64 boxes of 64 rows of w (128-byte swizzle);
-//                allocates TMEM
-//   warp 1       MMA issuer
-//   warps 2..17  scale and add: warp w owns TMEM lanes 32 (w % 4).. (rows) and
-//                the columns of part (w - 2) / 4 of the tile; writes the tile
-// The scales of the two chunks ahead are in registers before they are needed.
+//                and boxes of 64 rows of w (128-byte swizzle)
+//   warp 1       MMA issuer (the pair's first CTA)
+//   warp 2       allocates TMEM
+//   warp 3       loads the scales, four chunks at a time (4-byte cp.async:
+//                a segment's first row has any alignment)
+//   warps 4..19  scale and add: warp w owns TMEM lanes 32 (w % 4).. (rows) and
+//                the columns of part (w - 4) / 4 of the tile; writes the tile.
+//                They take the registers that the others do not need.
 // All waits are bounded (ts_common.cuh) and set the device error flag.
 #include "ts_fp8.cuh"
 #include "ts_kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ts {
 
@@ -34,35 +42,42 @@ int* fp8_err_flag() {
 }
 
 namespace f8 {
-constexpr uint32_t BM = 128;                  // rows of a per tile = TMEM lanes
-constexpr uint32_t A_BYTES = BM * kFp8Block;  // one chunk of a tile's rows
+constexpr uint32_t BM = 128;                  // rows of a per CTA = TMEM lanes
+constexpr uint32_t A_BYTES = BM * kFp8Block;  // one chunk of them
 constexpr uint32_t W_BOX = 64;                // rows of w per TMA box
 constexpr uint32_t TMEM_COLS = 512;
-constexpr uint32_t DRAIN_WARPS = 16;
-constexpr uint32_t THREADS = 32 * (2 + DRAIN_WARPS);
+constexpr uint32_t FIRST_DRAIN = 4, DRAIN_WARPS = 8;
+constexpr uint32_t THREADS = 32 * (FIRST_DRAIN + DRAIN_WARPS);
+// registers a thread: 168 at launch, moved to the warps that add
+constexpr uint32_t REGS_LAUNCH = 168, REGS_ROLES = 40, REGS_DRAIN = 232;
+static_assert(REGS_ROLES * 32 * FIRST_DRAIN + REGS_DRAIN * 32 * DRAIN_WARPS <= REGS_LAUNCH * THREADS, "register split");
 constexpr uint32_t MAX_E = 1024;
 constexpr uint32_t GROUP_M = 16;  // tiles of a that share their tiles of w in L2
+constexpr uint32_t BATCH = 4;     // chunks whose scales are loaded together
+constexpr uint32_t SB = 2;        // such batches in flight
 
-template <int BN>
+template <int CG, int BN, int WB>
 struct Cfg {
-  static constexpr uint32_t W_BYTES = BN * kFp8Block;
-  static constexpr uint32_t STAGE = A_BYTES + W_BYTES;
-  static constexpr uint32_t S = BN == 256 ? 3 : BN == 128 ? 4 : 6;
-  static constexpr uint32_t NB = TMEM_COLS / BN;      // TMEM buffers
-  static constexpr uint32_t PART = BN / 4;            // columns a warp owns
-  // a warp's rows on their way out: 32 of up to 128 bytes
-  static constexpr uint32_t OUT_BYTES = 32 * (PART * 4 < 128 ? PART * 4 : 128);
+  static constexpr uint32_t W_ROWS = BN / CG;  // rows of w that a CTA holds
+  static constexpr uint32_t STAGE = A_BYTES + W_ROWS * kFp8Block;
+  static constexpr uint32_t S = BN == 64 ? 6 : 4;
+  static constexpr uint32_t NB = TMEM_COLS / BN;  // TMEM buffers
+  static constexpr uint32_t PART = BN / 2;        // columns a warp owns
+  // a warp's rows on their way out: twice 32 of up to 128 bytes
+  static constexpr uint32_t OUT_BYTES = 2 * 32 * 128;
   static constexpr uint32_t OFF_OUT = S * STAGE;
-  static constexpr uint32_t OFF_BAR = OFF_OUT + DRAIN_WARPS * OUT_BYTES;
-  static constexpr uint32_t NUM_BARS = 2 * S + 2 * NB + 1;
+  // scales of a chunk: of the CTA's rows of a, then of the tile's columns, one
+  // for each (w_block 1) or for each 128
+  static constexpr uint32_t W_SCALES = WB == 1 ? BN : (BN + 127) / 128, SCALES = BM + (W_SCALES + 3) / 4 * 4;
+  static constexpr uint32_t OFF_SCALES = OFF_OUT + DRAIN_WARPS * OUT_BYTES;
+  static constexpr uint32_t OFF_BIAS = OFF_SCALES + SB * BATCH * SCALES * 4;  // a warp's columns' bias
+  static constexpr uint32_t OFF_BAR = OFF_BIAS + DRAIN_WARPS * PART * 4;
+  static constexpr uint32_t NUM_BARS = 2 * S + 2 * NB + 2 * SB + 1;
   static constexpr uint32_t OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr uint32_t OFF_SEG = OFF_MISC + 16;  // tile prefix of the segments, then their first rows
-  // the scales of a warp's columns, three chunks deep (w_block 1)
-  static constexpr uint32_t OFF_WS = (OFF_SEG + 16 + 15) / 16 * 16;
-  static constexpr uint32_t SMEM_SEG = OFF_SEG + (2 * MAX_E + 2) * 4 + 1024;
-  static constexpr uint32_t SMEM_ROW = OFF_WS + 3 * DRAIN_WARPS * PART * 4 + 1024;
+  static constexpr uint32_t SMEM = OFF_SEG + (WB == 1 ? 0 : (2 * MAX_E + 2) * 4) + 1024;
   static_assert(STAGE % 1024 == 0, "swizzle atoms");
-  static_assert(SMEM_SEG <= 227 * 1024 && SMEM_ROW <= 227 * 1024, "shared memory budget");
+  static_assert(OFF_BAR % 8 == 0 && SMEM <= 227 * 1024, "shared memory budget");
 };
 }  // namespace f8
 
@@ -70,47 +85,181 @@ struct Fp8Tile {
   uint32_t e, row0, row_end, n0;
 };
 
-// Tile t in an order that walks GROUP_M tiles of a for each tile of w.
-__device__ __forceinline__ Fp8Tile fp8_tile(const Fp8MmArgs& a, uint32_t t, uint32_t m_tiles, uint32_t n_tiles, uint32_t bn,
-                                            const uint32_t* pre, const int* first) {
-  const uint32_t per = f8::GROUP_M * n_tiles, g = t / per, r = t - g * per;
-  const uint32_t gm = min(f8::GROUP_M, m_tiles - g * f8::GROUP_M);
-  const uint32_t m = g * f8::GROUP_M + r % gm;
-  Fp8Tile ti;
-  ti.n0 = r / gm * bn;
-  if (a.seg) {
-    uint32_t lo = 0, hi = a.E;  // pre[lo] <= m < pre[hi]
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (pre[mid] <= m) lo = mid;
-      else hi = mid;
-    }
-    ti.e = lo;
-    ti.row0 = (uint32_t)first[lo] + (m - pre[lo]) * f8::BM;
-    ti.row_end = min(ti.row0 + f8::BM, (uint32_t)min(max(a.seg[lo + 1], 0), (int)a.M));
-  } else {
-    ti.e = 0;
-    ti.row0 = m * f8::BM;
-    ti.row_end = min(ti.row0 + f8::BM, a.M);
+// Walks the tiles of bm x bn that are `first`, `first + step`, ... in an order
+// that takes GROUP_M tiles of a for each tile of w.
+struct Fp8Walk {
+  uint32_t m_tiles, n_tiles, step, bm, bn;
+  uint32_t g, r;  // group of tiles of a, place in it
+
+  __device__ __forceinline__ Fp8Walk(uint32_t m_tiles_, uint32_t n_tiles_, uint32_t start, uint32_t step_, uint32_t bm_,
+                                     uint32_t bn_)
+      : m_tiles(m_tiles_), n_tiles(n_tiles_), step(step_), bm(bm_), bn(bn_), g(0), r(start) {
+    settle();
   }
-  return ti;
+  __device__ __forceinline__ uint32_t tiles_of_a() const { return min(f8::GROUP_M, m_tiles - g * f8::GROUP_M); }
+  __device__ __forceinline__ void settle() {
+    while (more() && r >= tiles_of_a() * n_tiles) {
+      r -= tiles_of_a() * n_tiles;
+      g++;
+    }
+  }
+  __device__ __forceinline__ bool more() const { return g * f8::GROUP_M < m_tiles; }
+  __device__ __forceinline__ void next() {
+    r += step;
+    settle();
+  }
+  __device__ __forceinline__ Fp8Tile tile(const Fp8MmArgs& a, const uint32_t* pre, const int* first) const {
+    const uint32_t gm = tiles_of_a(), n = gm == f8::GROUP_M ? r / f8::GROUP_M : r / gm, m = g * f8::GROUP_M + r - n * gm;
+    Fp8Tile ti;
+    ti.n0 = n * bn;
+    if (a.seg) {
+      uint32_t lo = 0, hi = a.E;  // pre[lo] <= m < pre[hi]
+      while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (pre[mid] <= m) lo = mid;
+        else hi = mid;
+      }
+      ti.e = lo;
+      ti.row0 = (uint32_t)first[lo] + (m - pre[lo]) * bm;
+      ti.row_end = min(ti.row0 + bm, (uint32_t)min(max(__ldg(&a.seg[lo + 1]), 0), (int)a.M));
+    } else {
+      ti.e = 0;
+      ti.row0 = m * bm;
+      ti.row_end = min(ti.row0 + bm, a.M);
+    }
+    return ti;
+  }
+};
+
+// --- PTX of single CTAs and of pairs (cta_group::2) ---
+template <uint32_t N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <uint32_t N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared-memory address of the same variable in the pair's first CTA.
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void fp8_tmem_alloc(uint32_t* slot, uint32_t cols) {
+  if constexpr (CG == 1) {
+    tmem_alloc(slot, cols);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void fp8_tmem_dealloc(uint32_t taddr, uint32_t cols) {
+  if constexpr (CG == 1) tmem_dealloc(taddr, cols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void fp8_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives on bar, in both CTAs of a pair, once the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void fp8_commit(uint64_t* bar) {
+  if constexpr (CG == 1) tc_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// The same for this CTA's barrier alone.
+template <int CG>
+__device__ __forceinline__ void fp8_commit_own(uint64_t* bar) {
+  if constexpr (CG == 1) tc_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// A tile into this CTA's shared memory; its bytes count on the barrier at bar
+// (of a pair: the first CTA's).
+template <int CG>
+__device__ __forceinline__ void fp8_load(void* dst, const void* tmap, int32_t c0, int32_t c1, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
 }
 
-__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                          uint32_t accumulate) {
+// 4 bytes to shared memory, asynchronously; the barrier gets this thread's
+// arrival once all its copies so far have landed.
+__device__ __forceinline__ void cp_async_4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// 32 lanes x 32 columns of f32 from TMEM; usable after fp8_ld_wait of them.
+__device__ __forceinline__ void fp8_ld(uint32_t addr, float (&r)[32]) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(addr)
       : "memory");
 }
-
-// 32 lanes x PART columns of f32 from TMEM.
-template <int N>
-__device__ __forceinline__ void fp8_tmem_ld(uint32_t addr, uint32_t (&r)[N]) {
-  if constexpr (N == 32) tmem_ld_32x32b_x32(addr, r);
-  else tmem_ld_32x32b_x16(addr, r);
+__device__ __forceinline__ void fp8_ld_wait(float (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+                 "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]),
+                 "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]),
+                 "+f"(r[30]), "+f"(r[31])
+               :
+               : "memory");
 }
 
 __device__ __forceinline__ void tma_store_2d(const void* tmap, const void* smem_src, int32_t c0, int32_t c1) {
@@ -127,8 +276,11 @@ __device__ __forceinline__ void tma_add_2d(const void* tmap, const void* smem_sr
                : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// The thread's bulk stores have read their shared memory.
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+// All but the last LEFT groups of the thread's bulk stores have read their shared memory.
+template <int LEFT>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
+}
 __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 template <int OT>
@@ -142,107 +294,106 @@ __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
   }
 }
 
-// 16 bytes of bias: the 8 columns from n.
-__device__ __forceinline__ void fp8_bias8(const __half* bias, uint32_t n, uint32_t N, float (&b)[8]) {
-  if (n + 8 <= N && !(reinterpret_cast<uintptr_t>(bias + n) & 15u)) {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(bias + n));
-    const __half* h = reinterpret_cast<const __half*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 8; i++) b[i] = __half2float(h[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) b[i] = n + i < N ? __half2float(bias[n + i]) : 0.0f;
-  }
-}
-
 // Writes a warp's 32 rows (from row, those below row_end) x PART columns (from
-// n), thread = row: acc + bias (+ what out holds).  The rows go through the
-// warp's shared memory, 16-byte pieces swizzled as a tensor map of that row
-// size has them, and leave by one TMA store where all 32 rows are this tile's
-// (tma: out can be mapped), else row by row, consecutive lanes on consecutive
-// columns.
+// n), thread = row: acc + bias (f32 in shared memory, or null) (+ what out
+// holds).  The rows go through the warp's shared memory, two turns of 32 x 128
+// bytes so that one is filled while the other leaves, their 16-byte pieces
+// swizzled as a tensor map of that row size has them, and leave by one TMA
+// store where all 32 rows are this tile's (tma: out can be mapped), else row
+// by row, consecutive lanes on consecutive columns.
 template <int OT, int PART>
-__device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap* tmap_o, bool tma, uint8_t* stage,
-                                          uint32_t e, uint32_t row, uint32_t row_end, uint32_t n,
-                                          const uint64_t (&acc)[PART / 2]) {
+__device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap* tmap_o, bool tma, uint8_t* stages,
+                                          uint32_t& turn, const float* bias, uint32_t row, uint32_t row_end, uint32_t n,
+                                          const float (&acc)[PART]) {
   using D = Fp8Type<OT>;
   using T = typename D::T;
   constexpr uint32_t RB = PART * sizeof(T) < 128 ? PART * sizeof(T) : 128;  // bytes of a staged row
   constexpr uint32_t COLS = RB / sizeof(T), PER = 16 / sizeof(T);
   const uint32_t lane = threadIdx.x & 31;
+  uint8_t* stage = stages;
   auto piece = [&](uint32_t r, uint32_t c) {  // piece c of staged row r
     return stage + r * RB + ((c ^ ((r * RB / 128) % (RB / 16))) * 16);
   };
   const bool whole = tma && row + 32 <= row_end;
 #pragma unroll
   for (uint32_t c0 = 0; c0 < PART; c0 += COLS) {
-    if (n + c0 >= a.N) break;
-    if (lane == 0) bulk_wait_read();
-    __syncwarp();
+    if (n + c0 < a.N) {
+      stage = stages + (turn++ & 1u) * (32 * 128);
+      if (lane == 0) bulk_wait_read<1>();  // the store before the last has left this turn's place
+      __syncwarp();
+      auto fill = [&](auto with_bias) {
 #pragma unroll
-    for (uint32_t c = 0; c < COLS; c += 8) {
-      float b[8] = {};
-      if (a.bias) fp8_bias8(reinterpret_cast<const __half*>(a.bias) + (uint64_t)e * a.N, n + c0 + c, a.N, b);
-      uint32_t w[8];
+        for (uint32_t c = 0; c < COLS; c += PER) {
+          float x[PER];
 #pragma unroll
-      for (uint32_t i = 0; i < 8; i += 2) {
-        float x0, x1;
-        f2unpack(acc[(c0 + c + i) / 2], x0, x1);
-        x0 += b[i];
-        x1 += b[i + 1];
-        if constexpr (OT == TS_DTYPE_F32) {
-          w[i] = __float_as_uint(x0);
-          w[i + 1] = __float_as_uint(x1);
-        } else {
-          w[i / 2] = fp8_out2<OT>(x0, x1);
+          for (uint32_t i = 0; i < PER; i += 4) {
+            float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if constexpr (with_bias()) b = *reinterpret_cast<const float4*>(bias + c0 + c + i);
+            x[i] = acc[c0 + c + i] + b.x;
+            x[i + 1] = acc[c0 + c + i + 1] + b.y;
+            x[i + 2] = acc[c0 + c + i + 2] + b.z;
+            x[i + 3] = acc[c0 + c + i + 3] + b.w;
+          }
+          uint4 w;
+          if constexpr (OT == TS_DTYPE_F32)
+            w = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+          else
+            w = make_uint4(fp8_out2<OT>(x[0], x[1]), fp8_out2<OT>(x[2], x[3]), fp8_out2<OT>(x[4], x[5]),
+                           fp8_out2<OT>(x[6], x[7]));
+          *reinterpret_cast<uint4*>(piece(lane, c / PER)) = w;
         }
-      }
-      *reinterpret_cast<uint4*>(piece(lane, c / PER)) = make_uint4(w[0], w[1], w[2], w[3]);
-      if constexpr (OT == TS_DTYPE_F32) *reinterpret_cast<uint4*>(piece(lane, c / PER + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
-    }
-    if (whole) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        if (OT == TS_DTYPE_F32 && a.accumulate) tma_add_2d(tmap_o, stage, (int32_t)(n + c0), (int32_t)row);
-        else tma_store_2d(tmap_o, stage, (int32_t)(n + c0), (int32_t)row);
-        bulk_commit();
-      }
-    } else {
-      __syncwarp();
-      for (uint32_t r = 0; r < 32 && row + r < row_end; r++) {
-        T* o = reinterpret_cast<T*>(a.out) + (uint64_t)(row + r) * a.ldo + n + c0;
-        for (uint32_t c = lane; c < COLS && n + c0 + c < a.N; c += 32) {
-          const T v = reinterpret_cast<const T*>(piece(r, c / PER))[c % PER];
-          if (OT == TS_DTYPE_F32 && a.accumulate) o[c] = D::down(D::up(v) + D::up(o[c]));
-          else o[c] = v;
+      };
+      if (bias) fill(std::true_type{});
+      else fill(std::false_type{});
+      if (whole) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (OT == TS_DTYPE_F32 && a.accumulate) tma_add_2d(tmap_o, stage, (int32_t)(n + c0), (int32_t)row);
+          else tma_store_2d(tmap_o, stage, (int32_t)(n + c0), (int32_t)row);
+          bulk_commit();
         }
+      } else {
+        if (lane == 0) bulk_commit();  // an empty group keeps the count
+        __syncwarp();
+        for (uint32_t r = 0; r < 32 && row + r < row_end; r++) {
+          T* o = reinterpret_cast<T*>(a.out) + (uint64_t)(row + r) * a.ldo + n + c0;
+          for (uint32_t c = lane; c < COLS && n + c0 + c < a.N; c += 32) {
+            const T v = reinterpret_cast<const T*>(piece(r, c / PER))[c % PER];
+            if (OT == TS_DTYPE_F32 && a.accumulate) o[c] = D::down(D::up(v) + D::up(o[c]));
+            else o[c] = v;
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
   }
 }
 
-template <int BN, int WB, int OT>
+template <int CG, int BN, int WB, int OT>
 __global__ void __launch_bounds__(f8::THREADS, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                     const __grid_constant__ CUtensorMap tmap_o, const Fp8MmArgs args, uint32_t n_tiles, uint32_t tma_out) {
   using namespace f8;
-  using C = Cfg<BN>;
+  using C = Cfg<CG, BN, WB>;
+  constexpr uint32_t TILE_M = CG * BM;
   extern __shared__ uint8_t smem_dyn[];
   pdl_trigger();
   pdl_wait();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // [S] a chunk of both operands landed
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // [S] a chunk of both operands landed (all CTAs')
   uint64_t* empty = full + C::S;                                   // [S] its MMAs completed
   uint64_t* acc_full = empty + C::S;                               // [NB] a chunk's product is in TMEM
-  uint64_t* acc_empty = acc_full + C::NB;                          // [NB] the 16 warps have read it
-  uint64_t* drain = acc_empty + C::NB;
+  uint64_t* acc_empty = acc_full + C::NB;                          // [NB] the adding warps (all CTAs') have read it
+  uint64_t* sc_full = acc_empty + C::NB;                           // [SB] a batch of scales landed
+  uint64_t* sc_empty = sc_full + SB;                               // [SB] the adding warps have read it
+  uint64_t* drain = sc_empty + SB;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   uint32_t* pre = reinterpret_cast<uint32_t*>(smem + C::OFF_SEG);  // [E + 1] tiles before each segment
   int* first = reinterpret_cast<int*>(pre + MAX_E + 1);            // [E] first row of each segment
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < C::S; i++) {
@@ -251,17 +402,18 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
     }
     for (uint32_t i = 0; i < C::NB; i++) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], DRAIN_WARPS);
+      mbar_init(&acc_empty[i], CG * DRAIN_WARPS);
+    }
+    for (uint32_t i = 0; i < SB; i++) {
+      mbar_init(&sc_full[i], 32);
+      mbar_init(&sc_empty[i], DRAIN_WARPS);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
   }
-  if (warp == 0) {
-    tmem_alloc(tmem_slot, TMEM_COLS);
-    tmem_relinquish();
-  }
+  if (warp == 2) fp8_tmem_alloc<CG>(tmem_slot, TMEM_COLS);
   if (args.seg && warp == 1) {
     // tiles before each segment: lane l sums the tiles of segments 32 l ..
     uint32_t sum = 0;
@@ -271,7 +423,7 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
       const int lo = min(max(args.seg[e], 0), (int)args.M), hi = min(max(args.seg[e + 1], lo), (int)args.M);
       first[e] = lo;
       pre[e] = sum;
-      sum += (uint32_t)(hi - lo + (int)BM - 1) / BM;
+      sum += (uint32_t)(hi - lo + (int)TILE_M - 1) / TILE_M;
     }
     uint32_t incl = sum;
 #pragma unroll
@@ -287,190 +439,241 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // both CTAs' barriers are there
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t n_kc = fp8_blocks(args.K);
-  const uint32_t m_tiles = args.seg ? pre[args.E] : (args.M + BM - 1) / BM;
-  const uint32_t total = m_tiles * n_tiles;
+  const uint32_t m_tiles = args.seg ? pre[args.E] : (args.M + TILE_M - 1) / TILE_M;
+  Fp8Walk walk(m_tiles, n_tiles, blockIdx.x / CG, gridDim.x / CG, TILE_M, BN);
+  // the MMA's columns: those that the tile has, in steps of 16; a CTA of a pair holds half
+  auto columns = [&](uint32_t n0) { return (min((uint32_t)BN, args.N - n0) + 15u) & ~15u; };
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < (int)FIRST_DRAIN) {  // a warpgroup changes its registers as one
+    regs_dec<REGS_ROLES>();
+    if (warp == 0) {
+      if (lane == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (; walk.more() && ok; walk.next()) {
+          const Fp8Tile ti = walk.tile(args, pre, first);
+          const uint32_t held = columns(ti.n0) / CG, boxes = (held + W_BOX - 1) / W_BOX;
+          const int32_t wrow = (int32_t)(ti.e * args.N + ti.n0 + rank * held), arow = (int32_t)(ti.row0 + rank * BM);
+          for (uint32_t kc = 0; kc < n_kc; kc++, it++) {
+            const uint32_t s = it % C::S, u = it / C::S;
+            if (!wait_or_abort(&empty[s], (u & 1u) ^ 1u, args.err, abort_flag)) {
+              ok = false;
+              break;
+            }
+            uint8_t* st = smem + s * C::STAGE;
+            const uint32_t bar = CG == 2 ? leader_addr(&full[s]) : smem_u32(&full[s]);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * (A_BYTES + boxes * W_BOX * kFp8Block));
+            fp8_load<CG>(st, &tmap_a, (int32_t)(kc * kFp8Block), arow, bar);
+            for (uint32_t b = 0; b < boxes; b++)
+              fp8_load<CG>(st + A_BYTES + b * W_BOX * kFp8Block, &tmap_w, (int32_t)(kc * kFp8Block),
+                           wrow + (int32_t)(b * W_BOX), bar);
+          }
+        }
+        if (!ok && rank == 0)  // the copies in flight land before this CTA's shared memory goes
+          for (uint32_t j = it > C::S ? it - C::S : 0u; j < it; j++) mbar_wait(&full[j % C::S], (j / C::S) & 1u, args.err);
+        // every signal that the pair's first CTA sends to these barriers has come
+        if (ok && CG == 2)
+          for (uint32_t j = it > C::S ? it - C::S : 0u; j < it; j++)
+            if (!wait_or_abort(&empty[j % C::S], (j / C::S) & 1u, args.err, abort_flag)) break;
+      }
+    } else if (warp == 1 && rank == 0) {
+      const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), wdesc0 = umma_desc_sw128(smem_u32(smem + A_BYTES));
       uint32_t it = 0;
       bool ok = true;
-      for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        const Fp8Tile ti = fp8_tile(args, t, m_tiles, n_tiles, BN, pre, first);
-        const uint32_t boxes = (min((uint32_t)BN, args.N - ti.n0) + W_BOX - 1) / W_BOX;
-        const int32_t wrow = (int32_t)(ti.e * args.N + ti.n0);
+      for (; walk.more() && ok; walk.next()) {
+        const Fp8Tile ti = walk.tile(args, pre, first);
+        const uint32_t idesc = umma_idesc_f16_f32(TILE_M, columns(ti.n0));
         for (uint32_t kc = 0; kc < n_kc; kc++, it++) {
-          const uint32_t s = it % C::S, u = it / C::S;
-          if (!wait_or_abort(&empty[s], (u & 1u) ^ 1u, args.err, abort_flag)) {
-            ok = false;
-            break;
+          const uint32_t s = it % C::S, b = it % C::NB;
+          ok = __all_sync(0xffffffffu, wait_or_abort(&acc_empty[b], ((it / C::NB) & 1u) ^ 1u, args.err, abort_flag) &&
+                                           wait_or_abort(&full[s], (it / C::S) & 1u, args.err, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t off = (uint64_t)(s * (C::STAGE >> 4));
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++)  // 32 k = 32 bytes = 2 descriptor units
+              fp8_mma<CG>(tmem_base + b * BN, adesc0 + off + 2u * k, wdesc0 + off + 2u * k, idesc, k != 0);
+            fp8_commit<CG>(&empty[s]);
+            fp8_commit<CG>(&acc_full[b]);
           }
-          uint8_t* st = smem + s * C::STAGE;
-          mbar_arrive_expect_tx(&full[s], A_BYTES + boxes * W_BOX * kFp8Block);
-          tma_load_2d(st, &tmap_a, (int32_t)(kc * kFp8Block), (int32_t)ti.row0, &full[s]);
-          for (uint32_t b = 0; b < boxes; b++)
-            tma_load_2d(st + A_BYTES + b * W_BOX * kFp8Block, &tmap_w, (int32_t)(kc * kFp8Block),
-                        wrow + (int32_t)(b * W_BOX), &full[s]);
+          __syncwarp();
         }
       }
-      if (!ok)  // the copies in flight land before this CTA's shared memory goes
-        for (uint32_t j = it > C::S ? it - C::S : 0u; j < it; j++) mbar_wait(&full[j % C::S], (j / C::S) & 1u, args.err);
-    }
-  } else if (warp == 1) {
-    const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), wdesc0 = umma_desc_sw128(smem_u32(smem + A_BYTES));
-    uint32_t it = 0;
-    bool ok = true;
-    for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      const Fp8Tile ti = fp8_tile(args, t, m_tiles, n_tiles, BN, pre, first);
-      // as many columns as the tile has, in steps of 16
-      const uint32_t idesc = umma_idesc_f16_f32(BM, (min((uint32_t)BN, args.N - ti.n0) + 15u) & ~15u);
-      for (uint32_t kc = 0; kc < n_kc; kc++, it++) {
-        const uint32_t s = it % C::S, b = it % C::NB;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&acc_empty[b], ((it / C::NB) & 1u) ^ 1u, args.err, abort_flag) &&
-                                         wait_or_abort(&full[s], (it / C::S) & 1u, args.err, abort_flag));
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t off = (uint64_t)(s * (C::STAGE >> 4));
-#pragma unroll
-          for (uint32_t k = 0; k < 4; k++)  // 32 k = 32 bytes = 2 descriptor units
-            tc_mma_f8(tmem_base + b * BN, adesc0 + off + 2u * k, wdesc0 + off + 2u * k, idesc, k != 0);
-          tc_commit(&empty[s]);
-          tc_commit(&acc_full[b]);
-        }
-        __syncwarp();
-      }
-    }
-    if (elect_one()) tc_commit(drain);
-    __syncwarp();
-    if (lane == 0) mbar_wait(drain, 0, args.err);
-  } else {
-    constexpr int PART = (int)C::PART, LD = PART == 32 ? 32 : 16;
-    const uint32_t q = (uint32_t)(warp & 3), p = (uint32_t)(warp - 2) >> 2;
-    const uint32_t taddr = tmem_base + ((q * 32u) << 16) + p * PART;
-    const uint32_t nb = fp8_blocks(args.N);
-    uint8_t* stage = smem + C::OFF_OUT + (warp - 2) * C::OUT_BYTES;
-    // scales of row m and of column block (or columns) n, chunk c
-    float* ring = reinterpret_cast<float*>(smem + C::OFF_WS) + (warp - 2) * PART;
-    auto a_scale = [&](uint32_t m, uint32_t c) { return args.as[c * args.ldas + min(m, args.M - 1)]; };
-    auto w_scale = [&](const Fp8Tile& ti, uint32_t c) {
-      const uint32_t n = min(ti.n0 + p * PART, args.N - 1);
-      return args.ws[((uint64_t)ti.e * nb + n / kFp8Block) * n_kc + c];
-    };
-    auto w_rows = [&](const Fp8Tile& ti, uint32_t c) {  // into slot c % 3 of this warp's ring
-#pragma unroll
-      for (int j = lane; j < PART; j += 32)
-        ring[(c % 3) * DRAIN_WARPS * PART + j] = args.ws[c * args.ldws + min(ti.n0 + p * PART + j, args.N - 1)];
-    };
-    float a0 = 0, a1 = 0, w0 = 0, w1 = 0;
-    auto ahead = [&](const Fp8Tile& ti) {  // the first two chunks of a tile
-      const uint32_t m = ti.row0 + q * 32u + lane;
-      a0 = a_scale(m, 0);
-      a1 = n_kc > 1 ? a_scale(m, 1) : 0.0f;
-      if constexpr (WB == 1) {
-        __syncwarp();
-        w_rows(ti, 0);
-        if (n_kc > 1) w_rows(ti, 1);
-      } else {
-        w0 = w_scale(ti, 0);
-        w1 = n_kc > 1 ? w_scale(ti, 1) : 0.0f;
-      }
-    };
-    Fp8Tile ti{};
-    if (blockIdx.x < total) {
-      ti = fp8_tile(args, blockIdx.x, m_tiles, n_tiles, BN, pre, first);
-      ahead(ti);
-    }
-    uint32_t it = 0;
-    for (uint32_t t = blockIdx.x; t < total; t += gridDim.x) {
-      const uint32_t m = ti.row0 + q * 32u + lane;
-      uint64_t acc[PART / 2];
-#pragma unroll
-      for (int j = 0; j < PART / 2; j++) acc[j] = 0;
+      if (elect_one()) fp8_commit_own<CG>(drain);
+      __syncwarp();
+      if (lane == 0) mbar_wait(drain, 0, args.err);
+    } else if (warp == 3) {
+      const uint32_t nb = fp8_blocks(args.N);
+      uint32_t batch = 0;
       bool ok = true;
-      for (uint32_t kc = 0; kc < n_kc; kc++, it++) {
-        const uint32_t b = it % C::NB;
-        const float s = WB == 1 ? a0 : a0 * w0;
-        const uint64_t s2 = f2pack(s, s);
-        a0 = a1;
-        w0 = w1;
-        if (kc + 2 < n_kc) {
-          a1 = a_scale(m, kc + 2);
-          if constexpr (WB != 1) w1 = w_scale(ti, kc + 2);
-        }
-        if constexpr (WB == 1) {
-          __syncwarp();  // slot kc % 3 is written, slot (kc + 2) % 3 has been read
-          if (kc + 2 < n_kc) w_rows(ti, kc + 2);
-        }
-        if (!wait_or_abort(&acc_full[b], (it / C::NB) & 1u, args.err, abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < PART; c += LD) {
-          uint32_t r[LD];
-          fp8_tmem_ld<LD>(taddr + b * BN + c, r);
-          tmem_ld_wait();
-          if (c + LD >= PART) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[b]);
-          }
-#pragma unroll
-          for (int j = 0; j < LD; j += 2) {
-            uint64_t v = f2pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+      for (; walk.more() && ok; walk.next()) {
+        const Fp8Tile ti = walk.tile(args, pre, first);
+        const uint32_t row = ti.row0 + rank * BM;
+        for (uint32_t k0 = 0; k0 < n_kc; k0 += BATCH, batch++) {
+          const uint32_t sl = batch % SB;
+          ok = __all_sync(0xffffffffu, wait_or_abort(&sc_empty[sl], ((batch / SB) & 1u) ^ 1u, args.err, abort_flag));
+          if (!ok) break;
+          float* dst = reinterpret_cast<float*>(smem + C::OFF_SCALES) + sl * BATCH * C::SCALES;
+          for (uint32_t kc = k0; kc < min(n_kc, k0 + BATCH); kc++, dst += C::SCALES) {
+            const float* as = args.as + (uint64_t)kc * args.ldas;
+            for (uint32_t j = lane; j < BM; j += 32) cp_async_4(dst + j, as + min(row + j, args.M - 1));
             if constexpr (WB == 1) {
-              const float2 w = *reinterpret_cast<const float2*>(ring + (kc % 3) * DRAIN_WARPS * PART + c + j);
-              v = mul_f32x2(v, f2pack(w.x, w.y));
+              const float* ws = args.ws + (uint64_t)kc * args.ldws;
+              for (uint32_t j = lane; j < BN; j += 32) cp_async_4(dst + BM + j, ws + min(ti.n0 + j, args.N - 1));
+            } else if (lane < C::W_SCALES) {
+              const uint32_t n = min(ti.n0 / kFp8Block + lane, nb - 1);
+              cp_async_4(dst + BM + lane, args.ws + ((uint64_t)ti.e * nb + n) * n_kc + kc);
             }
-            acc[(c + j) / 2] = fma_f32x2(v, s2, acc[(c + j) / 2]);
           }
+          cp_async_arrive(&sc_full[sl]);
         }
       }
-      if (!ok) break;
-      const Fp8Tile done = ti;
-      if (t + gridDim.x < total) {
-        ti = fp8_tile(args, t + gridDim.x, m_tiles, n_tiles, BN, pre, first);
-        ahead(ti);
+      cp_async_wait_all();
+    }
+  } else {
+    regs_inc<REGS_DRAIN>();
+    constexpr int PART = (int)C::PART;
+    const uint32_t q = (uint32_t)(warp & 3), p = (uint32_t)(warp - (int)FIRST_DRAIN) >> 2;
+    const uint32_t taddr = tmem_base + ((q * 32u) << 16) + p * PART, mine = rank * BM + q * 32u;
+    uint8_t* stages = smem + C::OFF_OUT + (warp - (int)FIRST_DRAIN) * C::OUT_BYTES;
+    uint32_t turn = 0;
+    const uint32_t empty_addr = CG == 2 ? leader_addr(acc_empty) : smem_u32(acc_empty);
+    const float* const scales = reinterpret_cast<const float*>(smem + C::OFF_SCALES);
+    float* const bias = reinterpret_cast<float*>(smem + C::OFF_BIAS) + (warp - (int)FIRST_DRAIN) * PART;
+    uint32_t it = 0, batch = 0;
+    bool ok = true;  // after a wait that ran out: no more waits and no output
+    for (; walk.more() && ok; walk.next()) {
+      const Fp8Tile ti = walk.tile(args, pre, first);
+      const uint32_t n = ti.n0 + p * PART;
+      uint16_t b16[PART / 32];  // fp16 bias of columns lane, lane + 32, ..: on its way while the tile is summed
+      if (args.bias)
+#pragma unroll
+        for (int j = 0; j < PART / 32; j++)
+          b16[j] = __ldg(&args.bias[(uint64_t)ti.e * args.N + min(n + j * 32 + lane, args.N - 1)]);
+      float acc[PART];
+#pragma unroll
+      for (int j = 0; j < PART; j++) acc[j] = 0.0f;
+#pragma unroll 1
+      for (uint32_t kc = 0; kc < n_kc; kc++, it++) {
+        const uint32_t b = it % C::NB, sl = batch % SB, in_batch = kc % BATCH;
+        if (in_batch == 0 && ok) ok = wait_or_abort(&sc_full[sl], (batch / SB) & 1u, args.err, abort_flag);
+        const float* sc = scales + (sl * BATCH + in_batch) * C::SCALES;
+        float s = sc[q * 32u + lane];
+        if constexpr (WB != 1) s *= sc[BM + p * PART / 128];
+        if (ok) ok = wait_or_abort(&acc_full[b], (it / C::NB) & 1u, args.err, abort_flag);
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t src = taddr + b * BN;
+        float r0[32], r1[32];
+        auto add = [&](const float (&r)[32], int c) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) {
+            if constexpr (WB == 1) acc[c + j] = fmaf(r[j] * sc[BM + p * PART + c + j], s, acc[c + j]);
+            else acc[c + j] = fmaf(r[j], s, acc[c + j]);
+          }
+        };
+        auto release = [&]() {  // the buffer has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 2) mbar_arrive_cluster(empty_addr + b * 8);
+            else mbar_arrive(&acc_empty[b]);
+          }
+        };
+        // one load is on its way while the other's values are added
+        fp8_ld(src, r0);
+        fp8_ld_wait(r0);
+        if constexpr (PART >= 64) fp8_ld(src + 32, r1);
+        else release();
+        add(r0, 0);
+        if constexpr (PART >= 64) {
+          fp8_ld_wait(r1);
+          if constexpr (PART == 128) fp8_ld(src + 64, r0);
+          else release();
+          add(r1, 32);
+        }
+        if constexpr (PART == 128) {
+          fp8_ld_wait(r0);
+          fp8_ld(src + 96, r1);
+          add(r0, 64);
+          fp8_ld_wait(r1);
+          release();
+          add(r1, 96);
+        }
+        if (in_batch == BATCH - 1 || kc + 1 == n_kc) {  // the batch's scales have been read
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_empty[sl]);
+          batch++;
+        }
       }
-      fp8_write<OT, PART>(args, &tmap_o, tma_out, stage, done.e, done.row0 + q * 32u, done.row_end, done.n0 + p * PART, acc);
+      if (args.bias) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < PART / 32; j++) bias[j * 32 + lane] = __half2float(__ushort_as_half(b16[j]));
+        __syncwarp();
+      }
+      if (__all_sync(0xffffffffu, ok))
+        fp8_write<OT, PART>(args, &tmap_o, tma_out, stages, turn, args.bias ? bias : nullptr, ti.row0 + mine, ti.row_end, n,
+                            acc);
     }
     if (lane == 0) bulk_wait();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if constexpr (CG == 2) cluster_sync();  // no CTA leaves while the other may signal it or read its operands
+  if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    fp8_tmem_dealloc<CG>(tmem_base, TMEM_COLS);
   }
 }
 
-template <int BN, int WB, int OT>
+template <int CG, int BN, int WB, int OT>
 static cudaError_t launch_gemm(const CUtensorMap& ta, const CUtensorMap& tw, const Fp8MmArgs& a, uint64_t m_tiles,
                                cudaStream_t st) {
-  using C = f8::Cfg<BN>;
+  using C = f8::Cfg<CG, BN, WB>;
+  auto* kernel = fp8_gemm_kernel<CG, BN, WB, OT>;
   static std::atomic<uint64_t> attr_done{0};
-  constexpr uint32_t smem = WB == 1 ? C::SMEM_ROW : C::SMEM_SEG;
-  if (cudaError_t e = smem_attr_per_device(fp8_gemm_kernel<BN, WB, OT>, (int)smem, attr_done); e != cudaSuccess) return e;
+  constexpr uint32_t smem = C::SMEM;
+  if (cudaError_t e = smem_attr_per_device(kernel, (int)smem, attr_done); e != cudaSuccess) return e;
   const uint32_t n_tiles = (a.N + BN - 1) / BN;
-  const uint32_t grid = (uint32_t)std::min<uint64_t>(m_tiles * n_tiles, (uint64_t)num_sms());
+  const uint32_t grid = CG * (uint32_t)std::min<uint64_t>(m_tiles * n_tiles, (uint64_t)num_sms() / CG);
   // out as 16-byte pieces of rows that can be mapped: the tensor map's box is a
   // warp's 32 rows of up to 128 bytes
   constexpr uint32_t size = sizeof(typename Fp8Type<OT>::T), bytes = std::min<uint32_t>(C::PART * size, 128);
   CUtensorMap to = ta;
   const uint32_t tma_out = make_out_tmap(&to, a.out, OT, a.M, a.N, a.ldo, bytes / size, 32) ? 1 : 0;
-  return launch_pdl(fp8_gemm_kernel<BN, WB, OT>, dim3(grid), dim3(f8::THREADS), smem, st, ta, tw, to, a, n_tiles, tma_out);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(f8::THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = CG;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CG;  // single CTAs have no cluster
+  return cudaLaunchKernelEx(&cfg, kernel, ta, tw, to, a, n_tiles, tma_out);
 }
 
-template <int BN, int WB>
+template <int CG, int BN>
 static cudaError_t launch_gemm_out(const CUtensorMap& ta, const CUtensorMap& tw, const Fp8MmArgs& a, uint64_t m_tiles,
                                    cudaStream_t st) {
-  if (a.out_dtype == TS_DTYPE_F16) return launch_gemm<BN, WB, TS_DTYPE_F16>(ta, tw, a, m_tiles, st);
-  if (a.out_dtype == TS_DTYPE_BF16) return launch_gemm<BN, WB, TS_DTYPE_BF16>(ta, tw, a, m_tiles, st);
-  return launch_gemm<BN, WB, TS_DTYPE_F32>(ta, tw, a, m_tiles, st);
+  if (a.w_block == 1) {
+    if (a.out_dtype == TS_DTYPE_F16) return launch_gemm<CG, BN, 1, TS_DTYPE_F16>(ta, tw, a, m_tiles, st);
+    if (a.out_dtype == TS_DTYPE_BF16) return launch_gemm<CG, BN, 1, TS_DTYPE_BF16>(ta, tw, a, m_tiles, st);
+    return launch_gemm<CG, BN, 1, TS_DTYPE_F32>(ta, tw, a, m_tiles, st);
+  }
+  if (a.out_dtype == TS_DTYPE_F16) return launch_gemm<CG, BN, 128, TS_DTYPE_F16>(ta, tw, a, m_tiles, st);
+  if (a.out_dtype == TS_DTYPE_BF16) return launch_gemm<CG, BN, 128, TS_DTYPE_BF16>(ta, tw, a, m_tiles, st);
+  return launch_gemm<CG, BN, 128, TS_DTYPE_F32>(ta, tw, a, m_tiles, st);
 }
 
 // K = 0: bias or zero (+ what out holds) on the rows that a segment covers.
@@ -509,20 +712,16 @@ cudaError_t launch_fp8_matmul(const Fp8MmArgs& a, cudaStream_t st) {
   if (!make_codes_tmap(&ta, a.a, a.M, a.K, a.lda, f8::BM) ||
       !make_codes_tmap(&tw, a.w, (uint64_t)a.E * a.N, a.K, a.ldw, f8::W_BOX))
     return cudaErrorInvalidValue;
-  // tiles of a: exact without segments; with them, an upper bound of what
+  // tiles of bm rows: exact without segments; with them, an upper bound of what
   // M rows in E segments can make
-  const uint64_t m_tiles = a.seg ? a.M / f8::BM + std::min(a.E, a.M) : (a.M + f8::BM - 1) / f8::BM;
-  // the widest tile that still gives every SM one
-  const uint64_t sms = (uint64_t)num_sms();
-  auto fills = [&](uint32_t bn) { return m_tiles * ((a.N + bn - 1) / bn) >= sms; };
-  if (a.w_block == 1) {
-    if (fills(256)) return launch_gemm_out<256, 1>(ta, tw, a, m_tiles, st);
-    if (fills(128)) return launch_gemm_out<128, 1>(ta, tw, a, m_tiles, st);
-    return launch_gemm_out<64, 1>(ta, tw, a, m_tiles, st);
-  }
-  if (fills(256)) return launch_gemm_out<256, 128>(ta, tw, a, m_tiles, st);
-  if (fills(128)) return launch_gemm_out<128, 128>(ta, tw, a, m_tiles, st);
-  return launch_gemm_out<64, 128>(ta, tw, a, m_tiles, st);
+  auto m_tiles = [&](uint32_t bm) { return a.seg ? a.M / bm + std::min(a.E, a.M) : ((uint64_t)a.M + bm - 1) / bm; };
+  // the largest tile that still gives every SM one
+  auto fills = [&](uint32_t bm, uint32_t bn) {
+    return m_tiles(bm) * ((a.N + bn - 1) / bn) * (bm / f8::BM) >= (uint64_t)num_sms();
+  };
+  if (fills(256, 256)) return launch_gemm_out<2, 256>(ta, tw, a, m_tiles(256), st);
+  if (fills(128, 128)) return launch_gemm_out<1, 128>(ta, tw, a, m_tiles(128), st);
+  return launch_gemm_out<1, 64>(ta, tw, a, m_tiles(128), st);
 }
 
 }  // namespace ts
