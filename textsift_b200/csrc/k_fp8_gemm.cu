@@ -71,7 +71,7 @@ struct Cfg {
   static constexpr uint32_t W_SCALES = WB == 1 ? BN : (BN + 127) / 128, SCALES = BM + (W_SCALES + 3) / 4 * 4;
   static constexpr uint32_t OFF_SCALES = OFF_OUT + DRAIN_WARPS * OUT_BYTES;
   static constexpr uint32_t OFF_BIAS = OFF_SCALES + SB * BATCH * SCALES * 4;  // a warp's columns' bias
-  static constexpr uint32_t OFF_BAR = OFF_BIAS + DRAIN_WARPS * PART * 4;
+  static constexpr uint32_t OFF_BAR = OFF_BIAS + DRAIN_WARPS * PART * 2;
   static constexpr uint32_t NUM_BARS = 2 * S + 2 * NB + 2 * SB + 1;
   static constexpr uint32_t OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr uint32_t OFF_SEG = OFF_MISC + 16;  // tile prefix of the segments, then their first rows
@@ -228,6 +228,12 @@ __device__ __forceinline__ void fp8_load(void* dst, const void* tmap, int32_t c0
         : "memory");
 }
 
+// A load that stays where it is written.
+__device__ __forceinline__ uint16_t ld_u16(const uint16_t* p) {
+  uint16_t v;
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
+  return v;
+}
 // 4 bytes to shared memory, asynchronously; the barrier gets this thread's
 // arrival once all its copies so far have landed.
 __device__ __forceinline__ void cp_async_4(void* dst, const void* src) {
@@ -295,7 +301,7 @@ __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
 }
 
 // Writes a warp's 32 rows (from row, those below row_end) x PART columns (from
-// n), thread = row: acc + bias (f32 in shared memory, or null) (+ what out
+// n), thread = row: acc + bias (fp16 in shared memory, or null) (+ what out
 // holds).  The rows go through the warp's shared memory, two turns of 32 x 128
 // bytes so that one is filled while the other leaves, their 16-byte pieces
 // swizzled as a tensor map of that row size has them, and leave by one TMA
@@ -303,7 +309,7 @@ __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
 // by row, consecutive lanes on consecutive columns.
 template <int OT, int PART>
 __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap* tmap_o, bool tma, uint8_t* stages,
-                                          uint32_t& turn, const float* bias, uint32_t row, uint32_t row_end, uint32_t n,
+                                          uint32_t& turn, const __half* bias, uint32_t row, uint32_t row_end, uint32_t n,
                                           const float (&acc)[PART]) {
   using D = Fp8Type<OT>;
   using T = typename D::T;
@@ -325,14 +331,17 @@ __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap*
 #pragma unroll
         for (uint32_t c = 0; c < COLS; c += PER) {
           float x[PER];
+          uint32_t b2[PER / 2];  // a wide read by all lanes of one address costs its bytes: halves, not floats
+          if constexpr (with_bias()) {
+            if constexpr (PER == 8) *reinterpret_cast<uint4*>(b2) = *reinterpret_cast<const uint4*>(bias + c0 + c);
+            else *reinterpret_cast<uint2*>(b2) = *reinterpret_cast<const uint2*>(bias + c0 + c);
+          }
 #pragma unroll
-          for (uint32_t i = 0; i < PER; i += 4) {
-            float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if constexpr (with_bias()) b = *reinterpret_cast<const float4*>(bias + c0 + c + i);
+          for (uint32_t i = 0; i < PER; i += 2) {
+            float2 b = make_float2(0.0f, 0.0f);
+            if constexpr (with_bias()) b = __half22float2(*reinterpret_cast<const __half2*>(&b2[i / 2]));
             x[i] = acc[c0 + c + i] + b.x;
             x[i + 1] = acc[c0 + c + i + 1] + b.y;
-            x[i + 2] = acc[c0 + c + i + 2] + b.z;
-            x[i + 3] = acc[c0 + c + i + 3] + b.w;
           }
           uint4 w;
           if constexpr (OT == TS_DTYPE_F32)
@@ -544,7 +553,7 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
     uint32_t turn = 0;
     const uint32_t empty_addr = CG == 2 ? leader_addr(acc_empty) : smem_u32(acc_empty);
     const float* const scales = reinterpret_cast<const float*>(smem + C::OFF_SCALES);
-    float* const bias = reinterpret_cast<float*>(smem + C::OFF_BIAS) + (warp - (int)FIRST_DRAIN) * PART;
+    __half* const bias = reinterpret_cast<__half*>(smem + C::OFF_BIAS) + (warp - (int)FIRST_DRAIN) * PART;
     uint32_t it = 0, batch = 0;
     bool ok = true;  // after a wait that ran out: no more waits and no output
     for (; walk.more() && ok; walk.next()) {
@@ -554,7 +563,7 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
       if (args.bias)
 #pragma unroll
         for (int j = 0; j < PART / 32; j++)
-          b16[j] = __ldg(&args.bias[(uint64_t)ti.e * args.N + min(n + j * 32 + lane, args.N - 1)]);
+          b16[j] = ld_u16(&args.bias[(uint64_t)ti.e * args.N + min(n + j * 32 + lane, args.N - 1)]);
       float acc[PART];
 #pragma unroll
       for (int j = 0; j < PART; j++) acc[j] = 0.0f;
@@ -614,7 +623,7 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
       if (args.bias) {
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < PART / 32; j++) bias[j * 32 + lane] = __half2float(__ushort_as_half(b16[j]));
+        for (int j = 0; j < PART / 32; j++) bias[j * 32 + lane] = __ushort_as_half(b16[j]);
         __syncwarp();
       }
       if (__all_sync(0xffffffffu, ok))
