@@ -8,12 +8,20 @@
 // buffer of its own, out of a ring, and 16 warps add it, times its scale, to
 // accumulators that stay in registers for the whole tile (64 x f32 a thread
 // at the widest).  Thread = one row of a, so as is one value a thread and
-// chunk, and ws one value a warp.
+// chunk, and ws one value a warp.  Where w has a scale for each row (w_block
+// 1), that layout would read as many scales as it adds values, and reading one
+// address by all lanes costs its bytes 32 times; TMEM is then read in the 16 x
+// 8 fragments of an mma (FRAG): four rows and a quarter of the columns a
+// thread, a quarter of the scales.
 //
 // Large products run on CTA pairs (cta_group::2, CG = 2): 256 rows of a by 256
 // rows of w, each CTA holding its half of both in shared memory and 128 of the
 // rows in its TMEM, so a chunk costs 32 KB of copies a CTA instead of 48; the
 // others on single CTAs with 128 rows of a by 128 or 64 of w.
+//
+// Where the tiles are too few for the GPU and k is long, a cluster of 2, 4 or 8
+// CTAs shares a tile (SPLIT): each sums a range of its chunks, the sums meet in
+// distributed shared memory and are added in the order of the ranges.
 //
 // Persistent, warp-specialized, one CTA per SM:
 //   warp 0       TMA producer: per chunk a box of 128 rows x 128 bytes of a
@@ -146,7 +154,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 // Shared-memory address of the same variable in the pair's first CTA.
 __device__ __forceinline__ uint32_t leader_addr(const void* p) {
@@ -257,6 +265,21 @@ __device__ __forceinline__ void fp8_ld(uint32_t addr, float (&r)[32]) {
       : "r"(addr)
       : "memory");
 }
+// 16 lanes x 64 columns: thread t gets, of each 8 columns g, columns 2 (t % 4)
+// and + 1 of lane t / 4 in r[4 g], r[4 g + 1] and of lane t / 4 + 8 in the
+// next two.
+__device__ __forceinline__ void fp8_ld_frag(uint32_t addr, float (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(addr)
+      : "memory");
+}
 __device__ __forceinline__ void fp8_ld_wait(float (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
@@ -268,6 +291,9 @@ __device__ __forceinline__ void fp8_ld_wait(float (&r)[32]) {
                : "memory");
 }
 
+__device__ __forceinline__ void prefetch_tmap(const void* tmap) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
+}
 __device__ __forceinline__ void tma_store_2d(const void* tmap, const void* smem_src, int32_t c0, int32_t c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
                    reinterpret_cast<uint64_t>(tmap)),
@@ -301,13 +327,13 @@ __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
 }
 
 // Writes a warp's 32 rows (from row, those below row_end) x PART columns (from
-// n), thread = row: acc + bias (fp16 in shared memory, or null) (+ what out
+// n), thread = row (or fragments): acc + bias (fp16 in shared memory, or null) (+ what out
 // holds).  The rows go through the warp's shared memory, two turns of 32 x 128
 // bytes so that one is filled while the other leaves, their 16-byte pieces
 // swizzled as a tensor map of that row size has them, and leave by one TMA
 // store where all 32 rows are this tile's (tma: out can be mapped), else row
 // by row, consecutive lanes on consecutive columns.
-template <int OT, int PART>
+template <int OT, int PART, bool FRAG>
 __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap* tmap_o, bool tma, uint8_t* stages,
                                           uint32_t& turn, const __half* bias, uint32_t row, uint32_t row_end, uint32_t n,
                                           const float (&acc)[PART]) {
@@ -352,8 +378,25 @@ __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap*
           *reinterpret_cast<uint4*>(piece(lane, c / PER)) = w;
         }
       };
-      if (bias) fill(std::true_type{});
-      else fill(std::false_type{});
+      if constexpr (FRAG) {
+#pragma unroll
+        for (uint32_t c = 0; c < COLS; c += 8) {
+          const uint32_t col = c + (lane & 3) * 2;
+          const float2 b = bias ? make_float2(__half2float(bias[c0 + col]), __half2float(bias[c0 + col + 1]))
+                                : make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (uint32_t i = 0; i < 4; i++) {  // rows lane / 4, + 8, + 16, + 24
+            const float* v = &acc[((i >> 1) * (PART / 8) + (c0 + c) / 8) * 4 + (i & 1) * 2];
+            uint8_t* dst = piece(i * 8 + (lane >> 2), col / PER) + col % PER * sizeof(T);
+            if constexpr (OT == TS_DTYPE_F32) *reinterpret_cast<float2*>(dst) = make_float2(v[0] + b.x, v[1] + b.y);
+            else *reinterpret_cast<uint32_t*>(dst) = fp8_out2<OT>(v[0] + b.x, v[1] + b.y);
+          }
+        }
+      } else if (bias) {
+        fill(std::true_type{});
+      } else {
+        fill(std::false_type{});
+      }
       if (whole) {
         fence_proxy_async_smem();
         __syncwarp();
@@ -379,16 +422,67 @@ __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap*
   }
 }
 
-template <int CG, int BN, int WB, int OT>
+// Place of 16-byte piece c of a row of BN floats: the rows of eight lanes that
+// write the same piece lie in different banks.
+template <int BN>
+__device__ __forceinline__ uint32_t fp8_swizzle(uint32_t c, uint32_t row) {
+  return c ^ (row & 7u);
+}
+
+// Adds the cluster's sums of a tile (f32 [128][BN] at the start of each CTA's
+// shared memory) in the order of the CTAs; the adding warps of CTA `part` of
+// `parts` write 128 / parts of the rows.
+template <int BN, int OT>
+__device__ __forceinline__ void fp8_join(const Fp8MmArgs& a, const Fp8Tile& ti, const uint8_t* smem, uint32_t part,
+                                         uint32_t parts) {
+  using D = Fp8Type<OT>;
+  using T = typename D::T;
+  const uint32_t rows = f8::BM / parts, base = smem_u32(smem);
+  for (uint32_t i = threadIdx.x - 32 * f8::FIRST_DRAIN; i < rows * (BN / 4); i += 32 * f8::DRAIN_WARPS) {
+    const uint32_t r = part * rows + i / (BN / 4), c = i % (BN / 4), m = ti.row0 + r, n = ti.n0 + c * 4;
+    if (m >= ti.row_end || n >= a.N) continue;
+    float4 v[8];  // all on their way before the first is added
+#pragma unroll
+    for (uint32_t s = 0; s < 8; s++)
+      if (s < parts)
+        asm volatile(
+            "{\n\t.reg .b32 a;\n\t"
+            "mapa.shared::cluster.u32 a, %4, %5;\n\t"
+            "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+            : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
+            : "r"(base + (r * (BN / 4) + fp8_swizzle<BN>(c, r)) * 16), "r"(s)
+            : "memory");
+    float x[4] = {};
+#pragma unroll
+    for (uint32_t s = 0; s < 8; s++)
+      if (s < parts) {
+        x[0] += v[s].x;
+        x[1] += v[s].y;
+        x[2] += v[s].z;
+        x[3] += v[s].w;
+      }
+    T* o = reinterpret_cast<T*>(a.out) + (uint64_t)m * a.ldo + n;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+      if (n + j >= a.N) break;
+      float v = x[j];
+      if (a.bias) v += __half2float(__ushort_as_half(__ldg(&a.bias[(uint64_t)ti.e * a.N + n + j])));
+      if (OT == TS_DTYPE_F32 && a.accumulate) v += D::up(o[j]);
+      o[j] = D::down(v);
+    }
+  }
+}
+
+template <int CG, int BN, int WB, int OT, bool SPLIT>
 __global__ void __launch_bounds__(f8::THREADS, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
-                    const __grid_constant__ CUtensorMap tmap_o, const Fp8MmArgs args, uint32_t n_tiles, uint32_t tma_out) {
+                    const __grid_constant__ CUtensorMap tmap_o, const Fp8MmArgs args, uint32_t n_tiles, uint32_t tma_out, uint32_t split) {
   using namespace f8;
   using C = Cfg<CG, BN, WB>;
   constexpr uint32_t TILE_M = CG * BM;
+  static_assert(CG == 1 || !SPLIT, "a cluster is a pair or a split");
   extern __shared__ uint8_t smem_dyn[];
   pdl_trigger();
-  pdl_wait();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // [S] a chunk of both operands landed (all CTAs')
   uint64_t* empty = full + C::S;                                   // [S] its MMAs completed
@@ -423,6 +517,12 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
     fence_proxy_async_smem();
   }
   if (warp == 2) fp8_tmem_alloc<CG>(tmem_slot, TMEM_COLS);
+  if (warp == 3 && lane == 0) {
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_w);
+    if (tma_out) prefetch_tmap(&tmap_o);
+  }
+  pdl_wait();  // global memory from here on
   if (args.seg && warp == 1) {
     // tiles before each segment: lane l sums the tiles of segments 32 l ..
     uint32_t sum = 0;
@@ -452,8 +552,12 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t n_kc = fp8_blocks(args.K);
+  // this CTA's chunks
+  const uint32_t part = SPLIT ? cluster_rank() : 0, parts = SPLIT ? split : 1;
+  const uint32_t k_lo = SPLIT ? n_kc * part / parts : 0, k_hi = SPLIT ? n_kc * (part + 1) / parts : n_kc;
   const uint32_t m_tiles = args.seg ? pre[args.E] : (args.M + TILE_M - 1) / TILE_M;
-  Fp8Walk walk(m_tiles, n_tiles, blockIdx.x / CG, gridDim.x / CG, TILE_M, BN);
+  Fp8Walk walk(m_tiles, n_tiles, blockIdx.x / (CG * parts), gridDim.x / (CG * parts), TILE_M, BN);
+  const bool busy = walk.more();  // the same for all CTAs of a cluster
   // the MMA's columns: those that the tile has, in steps of 16; a CTA of a pair holds half
   auto columns = [&](uint32_t n0) { return (min((uint32_t)BN, args.N - n0) + 15u) & ~15u; };
 
@@ -467,7 +571,7 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
           const Fp8Tile ti = walk.tile(args, pre, first);
           const uint32_t held = columns(ti.n0) / CG, boxes = (held + W_BOX - 1) / W_BOX;
           const int32_t wrow = (int32_t)(ti.e * args.N + ti.n0 + rank * held), arow = (int32_t)(ti.row0 + rank * BM);
-          for (uint32_t kc = 0; kc < n_kc; kc++, it++) {
+          for (uint32_t kc = k_lo; kc < k_hi; kc++, it++) {
             const uint32_t s = it % C::S, u = it / C::S;
             if (!wait_or_abort(&empty[s], (u & 1u) ^ 1u, args.err, abort_flag)) {
               ok = false;
@@ -496,7 +600,7 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
       for (; walk.more() && ok; walk.next()) {
         const Fp8Tile ti = walk.tile(args, pre, first);
         const uint32_t idesc = umma_idesc_f16_f32(TILE_M, columns(ti.n0));
-        for (uint32_t kc = 0; kc < n_kc; kc++, it++) {
+        for (uint32_t kc = k_lo; kc < k_hi; kc++, it++) {
           const uint32_t s = it % C::S, b = it % C::NB;
           ok = __all_sync(0xffffffffu, wait_or_abort(&acc_empty[b], ((it / C::NB) & 1u) ^ 1u, args.err, abort_flag) &&
                                            wait_or_abort(&full[s], (it / C::S) & 1u, args.err, abort_flag));
@@ -523,12 +627,12 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
       for (; walk.more() && ok; walk.next()) {
         const Fp8Tile ti = walk.tile(args, pre, first);
         const uint32_t row = ti.row0 + rank * BM;
-        for (uint32_t k0 = 0; k0 < n_kc; k0 += BATCH, batch++) {
+        for (uint32_t k0 = k_lo; k0 < k_hi; k0 += BATCH, batch++) {
           const uint32_t sl = batch % SB;
           ok = __all_sync(0xffffffffu, wait_or_abort(&sc_empty[sl], ((batch / SB) & 1u) ^ 1u, args.err, abort_flag));
           if (!ok) break;
           float* dst = reinterpret_cast<float*>(smem + C::OFF_SCALES) + sl * BATCH * C::SCALES;
-          for (uint32_t kc = k0; kc < min(n_kc, k0 + BATCH); kc++, dst += C::SCALES) {
+          for (uint32_t kc = k0; kc < min(k_hi, k0 + BATCH); kc++, dst += C::SCALES) {
             const float* as = args.as + (uint64_t)kc * args.ldas;
             for (uint32_t j = lane; j < BM; j += 32) cp_async_4(dst + j, as + min(row + j, args.M - 1));
             if constexpr (WB == 1) {
@@ -544,9 +648,13 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
       }
       cp_async_wait_all();
     }
+    __syncwarp();
+    if (SPLIT && busy) cluster_sync();  // where the adding warps join the sums
   } else {
     regs_inc<REGS_DRAIN>();
     constexpr int PART = (int)C::PART;
+    constexpr bool FRAG = WB == 1;
+    static_assert(!FRAG || PART >= 64, "fragments of 64 columns");
     const uint32_t q = (uint32_t)(warp & 3), p = (uint32_t)(warp - (int)FIRST_DRAIN) >> 2;
     const uint32_t taddr = tmem_base + ((q * 32u) << 16) + p * PART, mine = rank * BM + q * 32u;
     uint8_t* stages = smem + C::OFF_OUT + (warp - (int)FIRST_DRAIN) * C::OUT_BYTES;
@@ -568,22 +676,43 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
 #pragma unroll
       for (int j = 0; j < PART; j++) acc[j] = 0.0f;
 #pragma unroll 1
-      for (uint32_t kc = 0; kc < n_kc; kc++, it++) {
-        const uint32_t b = it % C::NB, sl = batch % SB, in_batch = kc % BATCH;
+      for (uint32_t kc = k_lo; kc < k_hi; kc++, it++) {
+        const uint32_t b = it % C::NB, sl = batch % SB, in_batch = (kc - k_lo) % BATCH;
         if (in_batch == 0 && ok) ok = wait_or_abort(&sc_full[sl], (batch / SB) & 1u, args.err, abort_flag);
         const float* sc = scales + (sl * BATCH + in_batch) * C::SCALES;
-        float s = sc[q * 32u + lane];
-        if constexpr (WB != 1) s *= sc[BM + p * PART / 128];
+        float s[4];  // of the thread's row, or its fragments' four
+        if constexpr (FRAG) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[j] = sc[q * 32u + j * 8 + (lane >> 2)];
+        } else {
+          s[0] = sc[q * 32u + lane] * sc[BM + p * PART / 128];
+        }
         if (ok) ok = wait_or_abort(&acc_full[b], (it / C::NB) & 1u, args.err, abort_flag);
         __syncwarp();
         tc_fence_after();
         const uint32_t src = taddr + b * BN;
         float r0[32], r1[32];
-        auto add = [&](const float (&r)[32], int c) {
+        // load i of the buffer: 32 columns of all rows, or 64 of 16 rows
+        constexpr int LOADS = PART / 32;
+        auto load = [&](int i, float (&r)[32]) {
+          if constexpr (FRAG) fp8_ld_frag(src + ((uint32_t)(i / (LOADS / 2)) << 20) + i % (LOADS / 2) * 64, r);
+          else fp8_ld(src + i * 32, r);
+        };
+        auto add = [&](int i, const float (&r)[32]) {
+          if constexpr (FRAG) {
+            const int half = i / (LOADS / 2), c = i % (LOADS / 2) * 64;
+            float* to = &acc[(half * (PART / 8) + c / 8) * 4];
 #pragma unroll
-          for (int j = 0; j < 32; j++) {
-            if constexpr (WB == 1) acc[c + j] = fmaf(r[j] * sc[BM + p * PART + c + j], s, acc[c + j]);
-            else acc[c + j] = fmaf(r[j], s, acc[c + j]);
+            for (int g = 0; g < 8; g++) {
+              const float2 w = *reinterpret_cast<const float2*>(sc + BM + p * PART + c + g * 8 + (lane & 3) * 2);
+              to[4 * g] = fmaf(r[4 * g], w.x * s[2 * half], to[4 * g]);
+              to[4 * g + 1] = fmaf(r[4 * g + 1], w.y * s[2 * half], to[4 * g + 1]);
+              to[4 * g + 2] = fmaf(r[4 * g + 2], w.x * s[2 * half + 1], to[4 * g + 2]);
+              to[4 * g + 3] = fmaf(r[4 * g + 3], w.y * s[2 * half + 1], to[4 * g + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++) acc[i * 32 + j] = fmaf(r[j], s[0], acc[i * 32 + j]);
           }
         };
         auto release = [&]() {  // the buffer has been read
@@ -595,30 +724,43 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
           }
         };
         // one load is on its way while the other's values are added
-        fp8_ld(src, r0);
+        load(0, r0);
         fp8_ld_wait(r0);
-        if constexpr (PART >= 64) fp8_ld(src + 32, r1);
-        else release();
-        add(r0, 0);
-        if constexpr (PART >= 64) {
-          fp8_ld_wait(r1);
-          if constexpr (PART == 128) fp8_ld(src + 64, r0);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+          float(&now)[32] = i & 1 ? r1 : r0;
+          float(&next)[32] = i & 1 ? r0 : r1;
+          if (i + 1 < LOADS) load(i + 1, next);
           else release();
-          add(r1, 32);
+          add(i, now);
+          if (i + 1 < LOADS) fp8_ld_wait(next);
         }
-        if constexpr (PART == 128) {
-          fp8_ld_wait(r0);
-          fp8_ld(src + 96, r1);
-          add(r0, 64);
-          fp8_ld_wait(r1);
-          release();
-          add(r1, 96);
-        }
-        if (in_batch == BATCH - 1 || kc + 1 == n_kc) {  // the batch's scales have been read
+        if (in_batch == BATCH - 1 || kc + 1 == k_hi) {  // the batch's scales have been read
           __syncwarp();
           if (lane == 0) mbar_arrive(&sc_empty[sl]);
           batch++;
         }
+      }
+      if constexpr (SPLIT) {
+        // the only tile of this CTA: its operands' shared memory is free now
+        if constexpr (FRAG) {
+#pragma unroll
+          for (int i = 0; i < PART / 2; i++) {  // pairs: half, 8 columns, upper or lower 8 rows
+            const uint32_t r = q * 32u + i / (PART / 4) * 16 + (i & 1) * 8 + (lane >> 2);
+            const uint32_t col = p * PART + i / 2 % (PART / 8) * 8 + (lane & 3) * 2;
+            float* dst = reinterpret_cast<float*>(smem) + (r * (BN / 4) + fp8_swizzle<BN>(col / 4, r)) * 4 + col % 4;
+            *reinterpret_cast<float2*>(dst) = make_float2(acc[2 * i], acc[2 * i + 1]);
+          }
+        } else {
+          float4* row = reinterpret_cast<float4*>(smem) + (q * 32u + lane) * (BN / 4);
+#pragma unroll
+          for (int j = 0; j < PART / 4; j++)
+            row[fp8_swizzle<BN>(p * (PART / 4) + j, lane)] =
+                make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+        }
+        cluster_sync();
+        if (ok) fp8_join<BN, OT>(args, ti, smem, part, parts);
+        break;
       }
       if (args.bias) {
         __syncwarp();
@@ -627,35 +769,36 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
         __syncwarp();
       }
       if (__all_sync(0xffffffffu, ok))
-        fp8_write<OT, PART>(args, &tmap_o, tma_out, stages, turn, args.bias ? bias : nullptr, ti.row0 + mine, ti.row_end, n,
+        fp8_write<OT, PART, FRAG>(args, &tmap_o, tma_out, stages, turn, args.bias ? bias : nullptr, ti.row0 + mine, ti.row_end, n,
                             acc);
     }
     if (lane == 0) bulk_wait();
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();  // no CTA leaves while the other may signal it or read its operands
+  if constexpr (CG == 2 || SPLIT) cluster_sync();  // no CTA leaves while the other may signal it or read its operands
   if (warp == 2) {
     tc_fence_after();
     fp8_tmem_dealloc<CG>(tmem_base, TMEM_COLS);
   }
 }
 
-template <int CG, int BN, int WB, int OT>
+template <int CG, int BN, int WB, int OT, bool SPLIT>
 static cudaError_t launch_gemm(const CUtensorMap& ta, const CUtensorMap& tw, const Fp8MmArgs& a, uint64_t m_tiles,
-                               cudaStream_t st) {
+                               uint32_t split, cudaStream_t st) {
   using C = f8::Cfg<CG, BN, WB>;
-  auto* kernel = fp8_gemm_kernel<CG, BN, WB, OT>;
+  auto* kernel = fp8_gemm_kernel<CG, BN, WB, OT, SPLIT>;
   static std::atomic<uint64_t> attr_done{0};
   constexpr uint32_t smem = C::SMEM;
   if (cudaError_t e = smem_attr_per_device(kernel, (int)smem, attr_done); e != cudaSuccess) return e;
-  const uint32_t n_tiles = (a.N + BN - 1) / BN;
-  const uint32_t grid = CG * (uint32_t)std::min<uint64_t>(m_tiles * n_tiles, (uint64_t)num_sms() / CG);
+  const uint32_t n_tiles = (a.N + BN - 1) / BN, cluster = CG * split;
+  const uint64_t tiles = m_tiles * n_tiles;
+  const uint32_t grid = cluster * (uint32_t)(SPLIT ? tiles : std::min<uint64_t>(tiles, (uint64_t)num_sms() / CG));
   // out as 16-byte pieces of rows that can be mapped: the tensor map's box is a
   // warp's 32 rows of up to 128 bytes
   constexpr uint32_t size = sizeof(typename Fp8Type<OT>::T), bytes = std::min<uint32_t>(C::PART * size, 128);
   CUtensorMap to = ta;
-  const uint32_t tma_out = make_out_tmap(&to, a.out, OT, a.M, a.N, a.ldo, bytes / size, 32) ? 1 : 0;
+  const uint32_t tma_out = !SPLIT && make_out_tmap(&to, a.out, OT, a.M, a.N, a.ldo, bytes / size, 32) ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(f8::THREADS);
@@ -665,24 +808,26 @@ static cudaError_t launch_gemm(const CUtensorMap& ta, const CUtensorMap& tw, con
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = CG;
+  at[1].val.clusterDim.x = cluster;
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = CG;  // single CTAs have no cluster
-  return cudaLaunchKernelEx(&cfg, kernel, ta, tw, to, a, n_tiles, tma_out);
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, ta, tw, to, a, n_tiles, tma_out, split);
 }
 
-template <int CG, int BN>
+template <int CG, int BN, bool SPLIT>
 static cudaError_t launch_gemm_out(const CUtensorMap& ta, const CUtensorMap& tw, const Fp8MmArgs& a, uint64_t m_tiles,
-                                   cudaStream_t st) {
-  if (a.w_block == 1) {
-    if (a.out_dtype == TS_DTYPE_F16) return launch_gemm<CG, BN, 1, TS_DTYPE_F16>(ta, tw, a, m_tiles, st);
-    if (a.out_dtype == TS_DTYPE_BF16) return launch_gemm<CG, BN, 1, TS_DTYPE_BF16>(ta, tw, a, m_tiles, st);
-    return launch_gemm<CG, BN, 1, TS_DTYPE_F32>(ta, tw, a, m_tiles, st);
+                                   uint32_t split, cudaStream_t st) {
+  if constexpr (BN >= 128) {
+    if (a.w_block == 1) {
+      if (a.out_dtype == TS_DTYPE_F16) return launch_gemm<CG, BN, 1, TS_DTYPE_F16, SPLIT>(ta, tw, a, m_tiles, split, st);
+      if (a.out_dtype == TS_DTYPE_BF16) return launch_gemm<CG, BN, 1, TS_DTYPE_BF16, SPLIT>(ta, tw, a, m_tiles, split, st);
+      return launch_gemm<CG, BN, 1, TS_DTYPE_F32, SPLIT>(ta, tw, a, m_tiles, split, st);
+    }
   }
-  if (a.out_dtype == TS_DTYPE_F16) return launch_gemm<CG, BN, 128, TS_DTYPE_F16>(ta, tw, a, m_tiles, st);
-  if (a.out_dtype == TS_DTYPE_BF16) return launch_gemm<CG, BN, 128, TS_DTYPE_BF16>(ta, tw, a, m_tiles, st);
-  return launch_gemm<CG, BN, 128, TS_DTYPE_F32>(ta, tw, a, m_tiles, st);
+  if (a.out_dtype == TS_DTYPE_F16) return launch_gemm<CG, BN, 128, TS_DTYPE_F16, SPLIT>(ta, tw, a, m_tiles, split, st);
+  if (a.out_dtype == TS_DTYPE_BF16) return launch_gemm<CG, BN, 128, TS_DTYPE_BF16, SPLIT>(ta, tw, a, m_tiles, split, st);
+  return launch_gemm<CG, BN, 128, TS_DTYPE_F32, SPLIT>(ta, tw, a, m_tiles, split, st);
 }
 
 // K = 0: bias or zero (+ what out holds) on the rows that a segment covers.
@@ -724,13 +869,38 @@ cudaError_t launch_fp8_matmul(const Fp8MmArgs& a, cudaStream_t st) {
   // tiles of bm rows: exact without segments; with them, an upper bound of what
   // M rows in E segments can make
   auto m_tiles = [&](uint32_t bm) { return a.seg ? a.M / bm + std::min(a.E, a.M) : ((uint64_t)a.M + bm - 1) / bm; };
-  // the largest tile that still gives every SM one
-  auto fills = [&](uint32_t bm, uint32_t bn) {
-    return m_tiles(bm) * ((a.N + bn - 1) / bn) * (bm / f8::BM) >= (uint64_t)num_sms();
+  // The form with the shortest estimate: rounds of tiles over the SMs, each
+  // `chunk` us for 128 of k (w_block 128, 1) and `tile` for the rest; the CTAs
+  // of a split do not outlive their tile, so a second round costs them a start.
+  // Measured, us, [pairs, 128, 64, 128 / 2, 128 / 4] at w_block 128:
+  //   8192 x 8192 x 8192   [546, 726, 1228, -, -]   1024 x 1024 x 8192  [40, 29, 27, 21, 27]
+  //   2048 x 2048 x 2048   [16, 19, 28, -, -]       128 x 4096 x 4096   [22, 16, 15, 14, 10]
+  //   512 x 640 x 640      [8.7, 6.8, 5.8, -, -]
+  // and 1280 x 640 x 16384 at w_block 1 [117, 80, -, 47, 53].
+  const uint64_t sms = (uint64_t)num_sms(), n_kc = fp8_blocks(a.K);
+  struct Form {
+    uint32_t cg, bn, split;
+    double chunk[2], tile;
   };
-  if (fills(256, 256)) return launch_gemm_out<2, 256>(ta, tw, a, m_tiles(256), st);
-  if (fills(128, 128)) return launch_gemm_out<1, 128>(ta, tw, a, m_tiles(128), st);
-  return launch_gemm_out<1, 64>(ta, tw, a, m_tiles(128), st);
+  static constexpr Form forms[] = {{2, 256, 1, {0.60, 0.92}, 1.1}, {1, 128, 1, {0.40, 0.60}, 1.0}, {1, 64, 1, {0.35, 0}, 0.6},
+                                   {1, 128, 2, {0.40, 0.60}, 3.5}, {1, 128, 4, {0.40, 0.60}, 3.5},
+                                   {1, 128, 8, {0.40, 0.60}, 3.5}};
+  const Form* best = nullptr;
+  double least = 0.0;
+  for (const Form& f : forms) {
+    if (f.split > n_kc || (f.bn < 128 && a.w_block == 1)) continue;
+    const uint64_t tiles = m_tiles(f.cg * f8::BM) * ((a.N + f.bn - 1) / f.bn), at_once = sms / (f.cg * f.split);
+    const uint64_t rounds = (tiles + at_once - 1) / at_once, chunks = (n_kc + f.split - 1) / f.split;
+    const double us = (double)rounds * ((double)chunks * f.chunk[a.w_block == 1] + f.tile) +
+                      (f.split > 1 ? (double)(rounds - 1) * 3.5 : 0.0);
+    if (!best || us < least) best = &f, least = us;
+  }
+  const uint64_t mt = m_tiles(best->cg * f8::BM);
+  if (best->cg == 2) return launch_gemm_out<2, 256, false>(ta, tw, a, mt, 1, st);
+  if (best->bn == 128)
+    return best->split == 1 ? launch_gemm_out<1, 128, false>(ta, tw, a, mt, 1, st)
+                            : launch_gemm_out<1, 128, true>(ta, tw, a, mt, best->split, st);
+  return launch_gemm_out<1, 64, false>(ta, tw, a, mt, 1, st);
 }
 
 }  // namespace ts
