@@ -408,13 +408,23 @@ __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap*
       } else {
         if (lane == 0) bulk_commit();  // an empty group keeps the count
         __syncwarp();
-        for (uint32_t r = 0; r < 32 && row + r < row_end; r++) {
-          T* o = reinterpret_cast<T*>(a.out) + (uint64_t)(row + r) * a.ldo + n + c0;
-          for (uint32_t c = lane; c < COLS && n + c0 + c < a.N; c += 32) {
-            const T v = reinterpret_cast<const T*>(piece(r, c / PER))[c % PER];
-            if (OT == TS_DTYPE_F32 && a.accumulate) o[c] = D::down(D::up(v) + D::up(o[c]));
-            else o[c] = v;
-          }
+        constexpr uint32_t AT_ONCE = 8, STEPS = (COLS + 31) / 32;  // rows on their way together
+        for (uint32_t r0 = 0; r0 < 32 && row + r0 < row_end; r0 += AT_ONCE) {
+          T v[AT_ONCE][STEPS];
+          T* o = reinterpret_cast<T*>(a.out) + (uint64_t)(row + r0) * a.ldo + n + c0;
+          auto each = [&](auto f) {
+#pragma unroll
+            for (uint32_t r = 0; r < AT_ONCE; r++)
+#pragma unroll
+              for (uint32_t j = 0; j < STEPS; j++) {
+                const uint32_t c = j * 32 + lane;
+                if (c < COLS && n + c0 + c < a.N && row + r0 + r < row_end) f(r, c, v[r][j]);
+              }
+          };
+          each([&](uint32_t r, uint32_t c, T& x) { x = reinterpret_cast<const T*>(piece(r0 + r, c / PER))[c % PER]; });
+          if (OT == TS_DTYPE_F32 && a.accumulate)
+            each([&](uint32_t r, uint32_t c, T& x) { x = D::down(D::up(x) + D::up(o[r * a.ldo + c])); });
+          each([&](uint32_t r, uint32_t c, T& x) { o[r * a.ldo + c] = x; });
         }
         __syncwarp();
       }

@@ -4,6 +4,9 @@
 // With a = max |x| over the finite values of a block: s = max(a * (1/448),
 // 2^-100), r = 1/s, code = e4m3(x * r), every f32 step rounded to nearest.
 #include "ts_fp8.cuh"
+#include "ts_kernels.h"
+
+#include <algorithm>
 
 namespace ts {
 
@@ -27,54 +30,100 @@ __global__ void __launch_bounds__(256, 8) fp8_quant_rows_kernel(const Fp8QuantAr
   if (c < a.cols) *reinterpret_cast<uint4*>(a.codes + row * a.ldc + c) = p.codes(fp8_inverse(s));
 }
 
-// A tile of 128 rows x 128 bytes (64 or 32 columns) through shared memory:
-// rows come in as they lie, and eight lanes then take one column (or, of
-// 16-bit types, two neighbours), 16 rows a lane, so that a column's 128 codes
-// leave as one line.  Four words after every 16 rows put the eight lanes'
-// rows into different banks.
+// Tiles of 128 rows x 128 bytes (64 or 32 columns) through shared memory: rows
+// come in as they lie, by cp.async, and eight lanes then take one column (or,
+// of 16-bit types, two neighbours), 16 rows a lane, so that a column's 128
+// codes leave as one line.  Four words after every 16 rows put the eight
+// lanes' rows into different banks.  The next tile is on its way while one is
+// quantised: with each block waiting for its own loads alone, DRAM was a
+// third as busy as it can be.
+namespace qc {
+constexpr uint32_t GROUP = 16 * 128 + 16;  // bytes of 16 rows
+constexpr uint32_t TILE = 8 * GROUP;
+constexpr uint32_t BLOCKS = 6;  // per SM: registers and shared memory allow as many
+}  // namespace qc
+
 template <int DT>
-__global__ void __launch_bounds__(256, 6) fp8_quant_cols_kernel(const Fp8QuantArgs a, uint32_t vec, uint32_t col_tiles) {
+__device__ __forceinline__ void fp8_cols_load(const Fp8QuantArgs& a, uint32_t vec, uint32_t b, uint32_t c0, uint8_t* tile) {
+  using D = Fp8Type<DT>;
+  using T = typename D::T;
+  const T* x = reinterpret_cast<const T*>(a.x);
+  if (vec) {
+    constexpr uint32_t PER = 16 / sizeof(T);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+      const uint32_t r = j * 32 + (threadIdx.x >> 3), o = (threadIdx.x & 7) * 16, c = c0 + o / sizeof(T);
+      const uint64_t row = (uint64_t)b * kFp8Block + r;
+      const uint32_t n = row < a.rows && c < a.cols ? min(PER, a.cols - c) : 0u;  // the rest becomes zeros
+      const T* src = n ? x + row * a.ldx + c : x;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                       smem_u32(tile + (r >> 4) * qc::GROUP + (r & 15) * 128 + o)),
+                   "l"(src), "r"(n * (uint32_t)sizeof(T))
+                   : "memory");
+    }
+  } else {
+    // value by value, a warp a row: 16 rows a warp, eight on their way together
+    constexpr uint32_t STEPS = 128 / sizeof(T) / 32;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (uint32_t r0 = 0; r0 < 16; r0 += 8) {
+      T v[8][STEPS];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; j++)
+#pragma unroll
+        for (uint32_t l = 0; l < STEPS; l++) {
+          const uint64_t row = (uint64_t)b * kFp8Block + warp * 16 + r0 + j;
+          const uint32_t c = c0 + l * 32 + lane;
+          v[j][l] = row < a.rows && c < a.cols ? x[row * a.ldx + c] : D::down(0.0f);
+        }
+#pragma unroll
+      for (uint32_t j = 0; j < 8; j++)
+#pragma unroll
+        for (uint32_t l = 0; l < STEPS; l++)
+          reinterpret_cast<T*>(tile + warp * qc::GROUP + (r0 + j) * 128)[l * 32 + lane] = v[j][l];
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256, qc::BLOCKS)
+    fp8_quant_cols_kernel(const Fp8QuantArgs a, uint32_t vec, uint32_t col_tiles, uint32_t tiles) {
   using D = Fp8Type<DT>;
   using T = typename D::T;
   constexpr uint32_t COLS = 128 / sizeof(T), W = sizeof(T) == 2 ? 2 : 1;  // columns a lane takes
-  constexpr uint32_t GROUP = 16 * 128 + 16;                               // bytes of 16 rows
-  __shared__ __align__(16) uint8_t tile[8 * GROUP];
+  __shared__ __align__(16) uint8_t tile[2][qc::TILE];
   pdl_trigger();
   pdl_wait();
-  const uint32_t b = blockIdx.x / col_tiles, c0 = blockIdx.x % col_tiles * COLS;
-  const T* x = reinterpret_cast<const T*>(a.x);
-#pragma unroll
-  for (uint32_t j = 0; j < 4; j++) {
-    const uint32_t r = j * 32 + (threadIdx.x >> 3), o = (threadIdx.x & 7) * 16;
-    const uint32_t c = c0 + o / sizeof(T);
-    const uint64_t row = (uint64_t)b * kFp8Block + r;
-    uint8_t* dst = tile + (r >> 4) * GROUP + (r & 15) * 128 + o;
-    constexpr uint32_t PER = 16 / sizeof(T);
-    if (vec && row < a.rows && c + PER <= a.cols) {
-      *reinterpret_cast<uint4*>(dst) = __ldg(reinterpret_cast<const uint4*>(x + row * a.ldx + c));
+  uint32_t turn = 0;
+  if (blockIdx.x < tiles) fp8_cols_load<DT>(a, vec, blockIdx.x / col_tiles, blockIdx.x % col_tiles * COLS, tile[0]);
+  for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, turn ^= 1) {
+    const uint32_t b = t / col_tiles, c0 = t % col_tiles * COLS, next = t + gridDim.x;
+    if (next < tiles) {
+      fp8_cols_load<DT>(a, vec, next / col_tiles, next % col_tiles * COLS, tile[turn ^ 1]);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
     } else {
-#pragma unroll
-      for (uint32_t l = 0; l < PER; l++)
-        reinterpret_cast<T*>(dst)[l] = row < a.rows && c + l < a.cols ? x[row * a.ldx + c + l] : D::down(0.0f);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-  }
-  __syncthreads();
-  const uint32_t col = threadIdx.x / 8 * W, g = threadIdx.x & 7;
-  const uint8_t* src = tile + g * GROUP + col * sizeof(T);
-  uint32_t raw[16];  // of both columns
+    __syncthreads();
+    const uint32_t col = threadIdx.x / 8 * W, g = threadIdx.x & 7;
+    const uint8_t* src = tile[turn] + g * qc::GROUP + col * sizeof(T);
+    uint32_t raw[16];  // of both columns
 #pragma unroll
-  for (uint32_t j = 0; j < 16; j++) raw[j] = *reinterpret_cast<const uint32_t*>(src + j * 128);
-  const uint32_t row0 = b * kFp8Block + g * 16;
+    for (uint32_t j = 0; j < 16; j++) raw[j] = *reinterpret_cast<const uint32_t*>(src + j * 128);
+    const uint32_t row0 = b * kFp8Block + g * 16;
 #pragma unroll
-  for (uint32_t w = 0; w < W; w++) {
-    Fp8Piece<DT> p;
+    for (uint32_t w = 0; w < W; w++) {
+      Fp8Piece<DT> p;
 #pragma unroll
-    for (uint32_t j = 0; j < 16; j++) p.v[j] = D::up(reinterpret_cast<const T*>(&raw[j])[w]);
-    const float s = fp8_scale(p.block_max());
-    const uint64_t c = c0 + col + w;
-    if (c >= a.cols) continue;
-    if (g == 0) a.scales[b * a.lds + c] = s;
-    if (row0 < a.rows) *reinterpret_cast<uint4*>(a.codes + c * a.ldc + row0) = p.codes(fp8_inverse(s));
+      for (uint32_t j = 0; j < 16; j++) p.v[j] = D::up(reinterpret_cast<const T*>(&raw[j])[w]);
+      const float s = fp8_scale(p.block_max());
+      const uint64_t c = c0 + col + w;
+      if (c >= a.cols) continue;
+      if (g == 0) a.scales[b * a.lds + c] = s;
+      if (row0 < a.rows) *reinterpret_cast<uint4*>(a.codes + c * a.ldc + row0) = p.codes(fp8_inverse(s));
+    }
+    __syncthreads();  // the tile's place is free for the load after the next
   }
 }
 
@@ -120,14 +169,15 @@ cudaError_t launch_fp8_quant_rows(const Fp8QuantArgs& a, cudaStream_t st) {
 
 cudaError_t launch_fp8_quant_cols(const Fp8QuantArgs& a, cudaStream_t st) {
   const uint32_t cols = a.dtype == TS_DTYPE_F32 ? 32 : 64, col_tiles = a.cols / cols + (a.cols % cols != 0);
-  const uint64_t grid = (uint64_t)col_tiles * fp8_blocks(a.rows);
-  if (grid > 0x7fffffffu) return cudaErrorInvalidValue;
-  const dim3 g((uint32_t)grid), t(256);
+  const uint64_t tiles = (uint64_t)col_tiles * fp8_blocks(a.rows);
+  if (tiles > 0x7fffffffu) return cudaErrorInvalidValue;
+  const dim3 g((uint32_t)std::min<uint64_t>(tiles, (uint64_t)num_sms() * qc::BLOCKS)), t(256);
+  const uint32_t n = (uint32_t)tiles;
   if (a.dtype == TS_DTYPE_F16)
-    return launch_pdl(fp8_quant_cols_kernel<TS_DTYPE_F16>, g, t, 0, st, a, fp8_vec(a), col_tiles);
+    return launch_pdl(fp8_quant_cols_kernel<TS_DTYPE_F16>, g, t, 0, st, a, fp8_vec(a), col_tiles, n);
   if (a.dtype == TS_DTYPE_BF16)
-    return launch_pdl(fp8_quant_cols_kernel<TS_DTYPE_BF16>, g, t, 0, st, a, fp8_vec(a), col_tiles);
-  return launch_pdl(fp8_quant_cols_kernel<TS_DTYPE_F32>, g, t, 0, st, a, fp8_vec(a), col_tiles);
+    return launch_pdl(fp8_quant_cols_kernel<TS_DTYPE_BF16>, g, t, 0, st, a, fp8_vec(a), col_tiles, n);
+  return launch_pdl(fp8_quant_cols_kernel<TS_DTYPE_F32>, g, t, 0, st, a, fp8_vec(a), col_tiles, n);
 }
 
 cudaError_t launch_fp8_transpose(const uint8_t* codes, uint64_t ldw, const float* scales, uint32_t E, uint32_t N,
