@@ -204,19 +204,20 @@ struct BalanceToken {
   static __device__ __forceinline__ uint32_t expert(int j) {
     return (uint32_t)((j / PER * L + (int)lane()) * PER + j % PER);
   }
-  __device__ __forceinline__ void load(const BalanceArgs& a, uint32_t t, bool vec) {
+  // `whole`: E = L V and rows start at multiples of 16 bytes
+  __device__ __forceinline__ void load(const BalanceArgs& a, uint32_t t, bool whole) {
     const T* x = static_cast<const T*>(a.logits) + t * a.ldl;
+    if (whole) {
+      const uint4* src = reinterpret_cast<const uint4*>(x) + lane();
 #pragma unroll
-    for (int j = 0; j < V; j += PER) {
-      const uint32_t e = expert(j);
-      if (vec && e + PER <= a.E) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x + e));
+      for (int j = 0; j < V / PER; j++) {
+        const uint4 raw = __ldg(src + j * L);
 #pragma unroll
-        for (int i = 0; i < PER; i++) z[j + i] = D::up(reinterpret_cast<const T*>(&raw)[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < PER; i++) z[j + i] = e + i < a.E ? D::up(x[e + i]) : -__int_as_float(0x7f800000);
+        for (int i = 0; i < PER; i++) z[j * PER + i] = D::up(reinterpret_cast<const T*>(&raw)[i]);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j++) z[j] = expert(j) < a.E ? D::up(x[expert(j)]) : -__int_as_float(0x7f800000);
     }
   }
   __device__ __forceinline__ void nothing() {
@@ -268,29 +269,26 @@ struct BalanceToken {
       }
     }
   }
-  __device__ __forceinline__ void write(const BalanceArgs& a, uint32_t t, const float (&cnt)[V], bool vec) const {
+  __device__ __forceinline__ void write(const BalanceArgs& a, uint32_t t, const float (&cnt)[V], bool whole) const {
     T* g = static_cast<T*>(a.grad) + t * a.ldg;
+    __align__(16) T out[V];
 #pragma unroll
-    for (int j = 0; j < V; j += PER) {
-      const uint32_t e = expert(j);
-      uint4 raw;
-      T* out = reinterpret_cast<T*>(&raw);
+    for (int j = 0; j < V; j++) out[j] = D::down(z[j] * fmaf(cnt[j], slope, base));
+    if (whole) {
+      uint4* dst = reinterpret_cast<uint4*>(g) + lane();
 #pragma unroll
-      for (int i = 0; i < PER; i++) out[i] = D::down(z[j + i] * fmaf(cnt[j + i], slope, base));
-      if (vec && e + PER <= a.E) {
-        *reinterpret_cast<uint4*>(g + e) = raw;
-      } else {
+      for (int j = 0; j < V / PER; j++) dst[j * L] = *reinterpret_cast<const uint4*>(&out[j * PER]);
+    } else {
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-          if (e + i < a.E) g[e + i] = out[i];
-      }
+      for (int j = 0; j < V; j++)
+        if (expert(j) < a.E) g[expert(j)] = out[j];
     }
   }
-  static __device__ __forceinline__ bool vec_in(const BalanceArgs& a) {
-    return !(reinterpret_cast<uintptr_t>(a.logits) & 15u) && a.ldl * sizeof(T) % 16 == 0;
+  static __device__ __forceinline__ bool whole_in(const BalanceArgs& a) {
+    return a.E == L * V && !(reinterpret_cast<uintptr_t>(a.logits) & 15u) && a.ldl * sizeof(T) % 16 == 0;
   }
-  static __device__ __forceinline__ bool vec_out(const BalanceArgs& a) {
-    return !(reinterpret_cast<uintptr_t>(a.grad) & 15u) && a.ldg * sizeof(T) % 16 == 0;
+  static __device__ __forceinline__ bool whole_out(const BalanceArgs& a) {
+    return a.E == L * V && !(reinterpret_cast<uintptr_t>(a.grad) & 15u) && a.ldg * sizeof(T) % 16 == 0;
   }
   // grad_scale alpha E / k for S' documents; over n twice for one of n tokens
   static __device__ __forceinline__ float factor(const BalanceArgs& a, int docs) {
@@ -298,12 +296,15 @@ struct BalanceToken {
   }
 };
 
+// Blocks of the kernel below that fit an SM (registers).
+__host__ __device__ constexpr int bal_blocks(int v) { return v <= 8 ? 4 : 1; }
+
 // A warp takes 32 / L tokens at once and `run` in a row for each lane group,
 // the next token's logits loaded while one is worked on; the group's document,
 // its counts and the sums of its probabilities stay in registers until the
 // document ends.
 template <int DT, int L, int V>
-__global__ void __launch_bounds__(bal::THREADS, V <= 8 ? 4 : 1) balance_tokens_kernel(const BalanceArgs a, uint32_t run) {
+__global__ void __launch_bounds__(bal::THREADS, bal_blocks(V)) balance_tokens_kernel(const BalanceArgs a, uint32_t run) {
   using namespace bal;
   using K = BalanceToken<DT, L, V>;
   __shared__ float red[WARPS][L * V];
@@ -311,12 +312,12 @@ __global__ void __launch_bounds__(bal::THREADS, V <= 8 ? 4 : 1) balance_tokens_k
   __shared__ int room[SEQ_SMEM];
   const BalanceWork w = balance_work(a);
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool vec_in = K::vec_in(a), vec_out = K::vec_out(a);
+  const bool whole_in = K::whole_in(a), whole_out = K::whole_out(a);
   const uint32_t first_t = (blockIdx.x * WARPS + warp) * run * K::GROUPS + K::group();
   K next;
   bool next_token = false;
   if (first_t < a.T) {
-    next.load(a, first_t, vec_in);
+    next.load(a, first_t, whole_in);
     next_token = balance_token(a, first_t);
   }
   const BalanceSeq q = balance_seq(a, room, SEQ_SMEM);
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(bal::THREADS, V <= 8 ? 4 : 1) balance_tokens_k
     K tok = next;
     const int s = next_token ? (t >= end ? q.doc(t) : now) : -1;
     if (i + 1 < run && t + K::GROUPS < a.T) {
-      next.load(a, t + K::GROUPS, vec_in);
+      next.load(a, t + K::GROUPS, whole_in);
       next_token = balance_token(a, t + K::GROUPS);
     }
     if (s >= 0) {
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(bal::THREADS, V <= 8 ? 4 : 1) balance_tokens_k
     } else {
       tok.nothing();
     }
-    if (a.grad) tok.write(a, t, cnt, vec_out);
+    if (a.grad) tok.write(a, t, cnt, whole_out);
   }
   // one row of sums a warp where all its groups hold the same document
   const int first = __shfl_sync(0xffffffffu, held, 0);
@@ -458,9 +459,9 @@ __global__ void __launch_bounds__(bal::ONE_THREADS, 1) balance_one_kernel(const 
   pdl_trigger();
   constexpr uint32_t STRIDE = ONE_THREADS / 32 * K::GROUPS;
   const uint32_t first_t = threadIdx.x / L;
-  const bool vec_in = K::vec_in(a), vec_out = K::vec_out(a);
+  const bool whole_in = K::whole_in(a), whole_out = K::whole_out(a);
   K next;
-  if (first_t < a.T) next.load(a, first_t, vec_in);
+  if (first_t < a.T) next.load(a, first_t, whole_in);
   const BalanceSeq q = balance_seq(a, m.seq, ONE_TABLE + 1);
   const uint32_t table = a.S * a.E;
   for (uint32_t i = threadIdx.x; i < table; i += ONE_THREADS) m.counts[i] = m.hi[i] = m.lo[i] = 0;
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__(bal::ONE_THREADS, 1) balance_one_kernel(const 
   const float all = K::factor(a, docs);
   for (uint32_t t = first_t; t < a.T; t += STRIDE) {
     K tok = next;
-    if (t + STRIDE < a.T) next.load(a, t + STRIDE, vec_in);
+    if (t + STRIDE < a.T) next.load(a, t + STRIDE, whole_in);
     const int s = m.doc[t];
     float cnt[V], psum[V];
 #pragma unroll
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(bal::ONE_THREADS, 1) balance_one_kernel(const 
     } else {
       tok.nothing();
     }
-    if (a.grad) tok.write(a, t, cnt, vec_out);
+    if (a.grad) tok.write(a, t, cnt, whole_out);
   }
   __syncthreads();
   double sum = 0.0;
@@ -535,8 +536,8 @@ static cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st) {
   const uint32_t count = (a.T + COUNT_TOKENS - 1) / COUNT_TOKENS;
   if (e == cudaSuccess && count) e = launch_pdl(balance_count_kernel, dim3(count), t, 0, st, a);
   if (e == cudaSuccess && a.T) {
-    // runs as long as four blocks an SM still have one
-    const uint32_t at_once = WARPS * (32 / L), wave = (uint32_t)num_sms() * 4 * at_once;
+    // runs as long as all blocks that fit the GPU still have one
+    const uint32_t at_once = WARPS * (32 / L), wave = (uint32_t)num_sms() * bal_blocks(V) * at_once;
     const uint32_t run = std::min(MAX_RUN, (a.T + wave - 1) / wave), tile = at_once * run;
     e = launch_pdl(balance_tokens_kernel<DT, L, V>, dim3((a.T + tile - 1) / tile), t, 0, st, a, run);
   }
@@ -544,6 +545,8 @@ static cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st) {
   return e;
 }
 
+// Eight values a lane: sixteen (eight lanes a token, half the instructions) need
+// so many registers that fewer blocks fit, 31 against 27 us at 65,536 x 128.
 template <int DT>
 static cudaError_t launch_balance_experts(const BalanceArgs& a, cudaStream_t st) {
   if (a.E <= 64) return launch_balance<DT, 8, 8>(a, st);
