@@ -218,3 +218,14 @@ def test_balance_repeats_bit_for_bit(cuda_lib):
         again, _ = balance(cuda_lib, z, F32, idx, mask, seq, st=st)
         for a, b in zip(first, again):
             assert np.array_equal(a, b)
+
+
+def test_balance_of_equal_counts(cuda_lib):
+    """Every expert takes every token: nothing to balance, a gradient of exactly zero and a loss of alpha."""
+    rng = np.random.default_rng(14)
+    for T, E in ((50, 4), (3000, 8)):
+        z = rng.standard_normal((T, E)).astype(np.float32) * 3
+        idx = np.tile(np.arange(E, dtype=np.int32), (T, 1))
+        got, _ = balance(cuda_lib, z, F32, idx, None, None, alpha=0.5)
+        assert (got[0] == T).all() and not got[3].any()
+        assert abs(got[2] - 0.5) <= 0.5 * (E + 16 + min(T, 1024)) * 2.0 ** -24

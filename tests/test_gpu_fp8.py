@@ -169,7 +169,39 @@ def test_matmul(cuda_lib, M, N, K, out):
     assert (o[:, N:].float() == -7.0).all()  # what lies between the rows stays
 
 
-@pytest.mark.parametrize("M,N,K", [(256, 256, 256), (1025, 1280, 640), (40, 640, 384)])
+# sizes that reach the CTA pairs (many tiles, their edges odd) and the clusters that split k (few tiles, k long)
+@pytest.mark.parametrize("M,N,K,out", [(9001, 2310, 385, F16), (9001, 2311, 385, BF16), (20000, 1152, 640, F16),
+                                       (6000, 3080, 129, F32), (100, 520, 4100, F16), (33, 64, 8192, F32),
+                                       (130, 127, 6001, BF16), (257, 1000, 2048, F32)])
+def test_matmul_large_and_long(cuda_lib, M, N, K, out):
+    rng = np.random.default_rng(M + N + K)
+    a, asc = f8.quant_rows(activations(rng, M, K))
+    w, ws = f8.quant_weight(rng.standard_normal((1, N, K)).astype(np.float32) / np.sqrt(K))
+    bias = (rng.standard_normal(N) * 0.1).astype(np.float16)
+    av, wv = f8.rows_value(a, asc), f8.weight_value(w[0], ws[0])
+    y = av @ wv.T + bias.astype(np.float64)
+    check(matmul(cuda_lib, a, asc, w, ws, M, N, K, out, bias=bias), av, wv, y, out, np.abs(bias.astype(np.float64)))
+
+
+@pytest.mark.parametrize("sizes,N,K", [([3000, 0, 5001, 17, 4100, 9000], 1032, 260), ([5, 0, 40, 1], 130, 4100),
+                                       ([0, 0, 0], 64, 4096)])
+def test_matmul_experts_large_and_long(cuda_lib, sizes, N, K):
+    E, M = len(sizes), max(1, sum(sizes))
+    rng = np.random.default_rng(M)
+    seg = np.concatenate([[0], np.cumsum(sizes)])
+    a, asc = f8.quant_rows(activations(rng, M, K))
+    w, ws = f8.quant_weight(rng.standard_normal((E, N, K)).astype(np.float32) / np.sqrt(K))
+    o = matmul(cuda_lib, a, asc, w, ws, M, N, K, F16, seg=seg, E=E)
+    av = f8.rows_value(a, asc)
+    for e in range(E):
+        r = slice(seg[e], seg[e + 1])
+        if sizes[e]:
+            wv = f8.weight_value(w[e], ws[e])
+            check(o[r], av[r], wv, av[r] @ wv.T, F16)
+    assert (o[seg[-1]:].float() == -7.0).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(256, 256, 256), (1025, 1280, 640), (40, 640, 384), (8192, 2304, 256), (64, 128, 4096)])
 def test_matmul_exact_integers(cuda_lib, M, N, K):
     """Small whole numbers and power-of-two scales leave nothing to round: every tile and block has to be exact."""
     rng = np.random.default_rng(K)
@@ -217,7 +249,8 @@ def test_matmul_rows_outside_segments_stay(cuda_lib):
     assert (o == -7.0).all()
 
 
-@pytest.mark.parametrize("T,N,K", [(1, 16, 16), (100, 130, 70), (129, 256, 128), (1000, 640, 1280), (4097, 64, 200)])
+@pytest.mark.parametrize("T,N,K", [(1, 16, 16), (100, 130, 70), (129, 256, 128), (1000, 640, 1280), (4097, 64, 200),
+                                   (260, 3001, 2050), (2050, 640, 1281)])
 def test_weight_gradient(cuda_lib, T, N, K):
     """dW = dY^T X from operands quantised along the tokens, written and accumulated."""
     rng = np.random.default_rng(T)
