@@ -272,6 +272,18 @@ def test_weight_gradient(cuda_lib, T, N, K):
     assert (np.abs(y - dyv.T.astype(np.float64) @ xv) <= 1.0001 * far).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(5, 130, 300), (16, 64, 128), (300, 257, 384), (300, 256, 129), (40, 64, 8192),
+                                   (9000, 2304, 130)])
+def test_accumulate(cuda_lib, M, N, K):
+    """Added to what the output holds, in every form of the product."""
+    rng = np.random.default_rng(M + K)
+    a, asc = f8.quant_rows(activations(rng, M, K))
+    w, ws = f8.quant_weight(rng.standard_normal((1, N, K)).astype(np.float32) / np.sqrt(K))
+    held = rng.standard_normal((M, N)).astype(np.float32)
+    av, wv = f8.rows_value(a, asc), f8.weight_value(w[0], ws[0])
+    check(matmul(cuda_lib, a, asc, w, ws, M, N, K, F32, acc=held), av, wv, av @ wv.T + held, F32, np.abs(held))
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 64, 128), (50, 300, 260), (300, 640, 1280)])
 def test_input_gradient(cuda_lib, M, N, K):
     """dX = dY W through the weight laid out by columns, against differences of the forward product: the product is

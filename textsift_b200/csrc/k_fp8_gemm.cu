@@ -332,7 +332,9 @@ __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
 // bytes so that one is filled while the other leaves, their 16-byte pieces
 // swizzled as a tensor map of that row size has them, and leave by one TMA
 // store where all 32 rows are this tile's (tma: out can be mapped), else row
-// by row, consecutive lanes on consecutive columns.
+// by row, consecutive lanes on consecutive columns.  (Measured at 65,536 x 1152
+// x 640: 80 us; the four warps of a column half behind one store of 128 rows 88
+// us; whole lines by ordinary stores from shared memory 98 us.)
 template <int OT, int PART, bool FRAG>
 __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap* tmap_o, bool tma, uint8_t* stages,
                                           uint32_t& turn, const __half* bias, uint32_t row, uint32_t row_end, uint32_t n,
