@@ -5,8 +5,8 @@
 // A block's scale multiplies the sum over its 128 k, so those 128 are one
 // accumulation of the tensor core (four tcgen05.mma.kind::f8f6f4 of 32 k) and
 // the sum over blocks is taken in registers: every chunk of 128 k has a TMEM
-// buffer of its own, out of a ring, and 16 warps add it, times its scale, to
-// accumulators that stay in registers for the whole tile (64 x f32 a thread
+// buffer of its own, out of a ring, and 8 warps add it, times its scale, to
+// accumulators that stay in registers for the whole tile (128 x f32 a thread
 // at the widest).  Thread = one row of a, so as is one value a thread and
 // chunk, and ws one value a warp.  Where w has a scale for each row (w_block
 // 1), that layout would read as many scales as it adds values, and reading one
@@ -30,8 +30,8 @@
 //   warp 2       allocates TMEM
 //   warp 3       loads the scales, four chunks at a time (4-byte cp.async:
 //                a segment's first row has any alignment)
-//   warps 4..19  scale and add: warp w owns TMEM lanes 32 (w % 4).. (rows) and
-//                the columns of part (w - 4) / 4 of the tile; writes the tile.
+//   warps 4..11  scale and add: warp w owns TMEM lanes 32 (w % 4).. (rows) and
+//                half (w - 4) / 4 of the tile's columns; writes the tile.
 //                They take the registers that the others do not need.
 // All waits are bounded (ts_common.cuh) and set the device error flag.
 #include "ts_fp8.cuh"
@@ -252,43 +252,82 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// 32 lanes x 32 columns of f32 from TMEM; usable after fp8_ld_wait of them.
-__device__ __forceinline__ void fp8_ld(uint32_t addr, float (&r)[32]) {
+// 32 lanes x N columns of f32 from TMEM, thread = lane.  The wait is part of
+// the load, so nothing can use the values before.
+template <int N>
+__device__ __forceinline__ void fp8_ld(uint32_t addr, float (&r)[N]);
+template <>
+__device__ __forceinline__ void fp8_ld<64>(uint32_t addr, float (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]),
+        "=f"(r[32]), "=f"(r[33]), "=f"(r[34]), "=f"(r[35]), "=f"(r[36]), "=f"(r[37]), "=f"(r[38]), "=f"(r[39]),
+        "=f"(r[40]), "=f"(r[41]), "=f"(r[42]), "=f"(r[43]), "=f"(r[44]), "=f"(r[45]), "=f"(r[46]), "=f"(r[47]),
+        "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
+        "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63])
+      : "r"(addr)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void fp8_ld<32>(uint32_t addr, float (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
       "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
-        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
-        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
       : "r"(addr)
       : "memory");
 }
-// 16 lanes x 64 columns: thread t gets, of each 8 columns g, columns 2 (t % 4)
+// 16 lanes x 2 N columns: thread t gets, of each 8 columns g, columns 2 (t % 4)
 // and + 1 of lane t / 4 in r[4 g], r[4 g + 1] and of lane t / 4 + 8 in the
 // next two.
-__device__ __forceinline__ void fp8_ld_frag(uint32_t addr, float (&r)[32]) {
+template <int N>
+__device__ __forceinline__ void fp8_ld_frag(uint32_t addr, float (&r)[N]);
+template <>
+__device__ __forceinline__ void fp8_ld_frag<64>(uint32_t addr, float (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x16.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]),
+        "=f"(r[32]), "=f"(r[33]), "=f"(r[34]), "=f"(r[35]), "=f"(r[36]), "=f"(r[37]), "=f"(r[38]), "=f"(r[39]),
+        "=f"(r[40]), "=f"(r[41]), "=f"(r[42]), "=f"(r[43]), "=f"(r[44]), "=f"(r[45]), "=f"(r[46]), "=f"(r[47]),
+        "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
+        "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63])
+      : "r"(addr)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void fp8_ld_frag<32>(uint32_t addr, float (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.16x256b.x8.b32 {"
       "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
-        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
-        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
       : "r"(addr)
       : "memory");
-}
-__device__ __forceinline__ void fp8_ld_wait(float (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
-                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
-                 "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]),
-                 "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]),
-                 "+f"(r[30]), "+f"(r[31])
-               :
-               : "memory");
 }
 
 __device__ __forceinline__ void prefetch_tmap(const void* tmap) {
@@ -703,30 +742,6 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
         __syncwarp();
         tc_fence_after();
         const uint32_t src = taddr + b * BN;
-        float r0[32], r1[32];
-        // load i of the buffer: 32 columns of all rows, or 64 of 16 rows
-        constexpr int LOADS = PART / 32;
-        auto load = [&](int i, float (&r)[32]) {
-          if constexpr (FRAG) fp8_ld_frag(src + ((uint32_t)(i / (LOADS / 2)) << 20) + i % (LOADS / 2) * 64, r);
-          else fp8_ld(src + i * 32, r);
-        };
-        auto add = [&](int i, const float (&r)[32]) {
-          if constexpr (FRAG) {
-            const int half = i / (LOADS / 2), c = i % (LOADS / 2) * 64;
-            float* to = &acc[(half * (PART / 8) + c / 8) * 4];
-#pragma unroll
-            for (int g = 0; g < 8; g++) {
-              const float2 w = *reinterpret_cast<const float2*>(sc + BM + p * PART + c + g * 8 + (lane & 3) * 2);
-              to[4 * g] = fmaf(r[4 * g], w.x * s[2 * half], to[4 * g]);
-              to[4 * g + 1] = fmaf(r[4 * g + 1], w.y * s[2 * half], to[4 * g + 1]);
-              to[4 * g + 2] = fmaf(r[4 * g + 2], w.x * s[2 * half + 1], to[4 * g + 2]);
-              to[4 * g + 3] = fmaf(r[4 * g + 3], w.y * s[2 * half + 1], to[4 * g + 3]);
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; j++) acc[i * 32 + j] = fmaf(r[j], s[0], acc[i * 32 + j]);
-          }
-        };
         auto release = [&]() {  // the buffer has been read
           tc_fence_before();
           __syncwarp();
@@ -735,17 +750,36 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
             else mbar_arrive(&acc_empty[b]);
           }
         };
-        // one load is on its way while the other's values are added
-        load(0, r0);
-        fp8_ld_wait(r0);
+        // as many columns a load as the registers hold beside the sums: the
+        // tensor core stands still while TMEM is read, the longer the more
+        // loads there are (32 columns each, one ahead of the adding: 451
+        // against 402 us for 128 experts)
+        if constexpr (FRAG) {
 #pragma unroll
-        for (int i = 0; i < LOADS; i++) {
-          float(&now)[32] = i & 1 ? r1 : r0;
-          float(&next)[32] = i & 1 ? r0 : r1;
-          if (i + 1 < LOADS) load(i + 1, next);
-          else release();
-          add(i, now);
-          if (i + 1 < LOADS) fp8_ld_wait(next);
+          for (int half = 0; half < 2; half++) {
+            float r[PART / 2];
+            fp8_ld_frag<PART / 2>(src + ((uint32_t)half << 20), r);
+            if (half == 1) release();
+            float* to = &acc[half * (PART / 2)];
+#pragma unroll
+            for (int g = 0; g < PART / 8; g++) {
+              const float2 w = *reinterpret_cast<const float2*>(sc + BM + p * PART + g * 8 + (lane & 3) * 2);
+              to[4 * g] = fmaf(r[4 * g], w.x * s[2 * half], to[4 * g]);
+              to[4 * g + 1] = fmaf(r[4 * g + 1], w.y * s[2 * half], to[4 * g + 1]);
+              to[4 * g + 2] = fmaf(r[4 * g + 2], w.x * s[2 * half + 1], to[4 * g + 2]);
+              to[4 * g + 3] = fmaf(r[4 * g + 3], w.y * s[2 * half + 1], to[4 * g + 3]);
+            }
+          }
+        } else {
+          constexpr int LD = PART < 64 ? PART : 64;
+#pragma unroll
+          for (int c = 0; c < PART; c += LD) {
+            float r[LD];
+            fp8_ld<LD>(src + c, r);
+            if (c + LD == PART) release();
+#pragma unroll
+            for (int j = 0; j < LD; j++) acc[c + j] = fmaf(r[j], s[0], acc[c + j]);
+          }
         }
         if (in_batch == BATCH - 1 || kc + 1 == k_hi) {  // the batch's scales have been read
           __syncwarp();
