@@ -38,7 +38,6 @@
 #include "ts_kernels.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace ts {
 
@@ -366,17 +365,17 @@ __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
 }
 
 // Writes a warp's 32 rows (from row, those below row_end) x PART columns (from
-// n), thread = row (or fragments): acc + bias (fp16 in shared memory, or null) (+ what out
-// holds).  The rows go through the warp's shared memory, two turns of 32 x 128
-// bytes so that one is filled while the other leaves, their 16-byte pieces
-// swizzled as a tensor map of that row size has them, and leave by one TMA
-// store where all 32 rows are this tile's (tma: out can be mapped), else row
-// by row, consecutive lanes on consecutive columns.  (Measured at 65,536 x 1152
-// x 640: 80 us; the four warps of a column half behind one store of 128 rows 88
-// us; whole lines by ordinary stores from shared memory 98 us.)
+// n), thread = row (or fragments): acc (+ what out holds).  The rows go through
+// the warp's shared memory, two turns of 32 x 128 bytes so that one is filled
+// while the other leaves, their 16-byte pieces swizzled as a tensor map of that
+// row size has them, and leave by one TMA store where all 32 rows are this
+// tile's (tma: out can be mapped), else row by row, consecutive lanes on
+// consecutive columns.  (Measured at 65,536 x 1152 x 640: 80 us; the four warps
+// of a column half behind one store of 128 rows 88 us; whole lines by ordinary
+// stores from shared memory 98 us.)
 template <int OT, int PART, bool FRAG>
 __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap* tmap_o, bool tma, uint8_t* stages,
-                                          uint32_t& turn, const __half* bias, uint32_t row, uint32_t row_end, uint32_t n,
+                                          uint32_t& turn, uint32_t row, uint32_t row_end, uint32_t n,
                                           const float (&acc)[PART]) {
   using D = Fp8Type<OT>;
   using T = typename D::T;
@@ -394,49 +393,30 @@ __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap*
       stage = stages + (turn++ & 1u) * (32 * 128);
       if (lane == 0) bulk_wait_read<1>();  // the store before the last has left this turn's place
       __syncwarp();
-      auto fill = [&](auto with_bias) {
-#pragma unroll
-        for (uint32_t c = 0; c < COLS; c += PER) {
-          float x[PER];
-          uint32_t b2[PER / 2];  // a wide read by all lanes of one address costs its bytes: halves, not floats
-          if constexpr (with_bias()) {
-            if constexpr (PER == 8) *reinterpret_cast<uint4*>(b2) = *reinterpret_cast<const uint4*>(bias + c0 + c);
-            else *reinterpret_cast<uint2*>(b2) = *reinterpret_cast<const uint2*>(bias + c0 + c);
-          }
-#pragma unroll
-          for (uint32_t i = 0; i < PER; i += 2) {
-            float2 b = make_float2(0.0f, 0.0f);
-            if constexpr (with_bias()) b = __half22float2(*reinterpret_cast<const __half2*>(&b2[i / 2]));
-            x[i] = acc[c0 + c + i] + b.x;
-            x[i + 1] = acc[c0 + c + i + 1] + b.y;
-          }
-          uint4 w;
-          if constexpr (OT == TS_DTYPE_F32)
-            w = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-          else
-            w = make_uint4(fp8_out2<OT>(x[0], x[1]), fp8_out2<OT>(x[2], x[3]), fp8_out2<OT>(x[4], x[5]),
-                           fp8_out2<OT>(x[6], x[7]));
-          *reinterpret_cast<uint4*>(piece(lane, c / PER)) = w;
-        }
-      };
       if constexpr (FRAG) {
 #pragma unroll
         for (uint32_t c = 0; c < COLS; c += 8) {
           const uint32_t col = c + (lane & 3) * 2;
-          const float2 b = bias ? make_float2(__half2float(bias[c0 + col]), __half2float(bias[c0 + col + 1]))
-                                : make_float2(0.0f, 0.0f);
 #pragma unroll
           for (uint32_t i = 0; i < 4; i++) {  // rows lane / 4, + 8, + 16, + 24
             const float* v = &acc[((i >> 1) * (PART / 8) + (c0 + c) / 8) * 4 + (i & 1) * 2];
             uint8_t* dst = piece(i * 8 + (lane >> 2), col / PER) + col % PER * sizeof(T);
-            if constexpr (OT == TS_DTYPE_F32) *reinterpret_cast<float2*>(dst) = make_float2(v[0] + b.x, v[1] + b.y);
-            else *reinterpret_cast<uint32_t*>(dst) = fp8_out2<OT>(v[0] + b.x, v[1] + b.y);
+            if constexpr (OT == TS_DTYPE_F32) *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
+            else *reinterpret_cast<uint32_t*>(dst) = fp8_out2<OT>(v[0], v[1]);
           }
         }
-      } else if (bias) {
-        fill(std::true_type{});
       } else {
-        fill(std::false_type{});
+#pragma unroll
+        for (uint32_t c = 0; c < COLS; c += PER) {
+          const float* v = &acc[c0 + c];
+          uint4 w;
+          if constexpr (OT == TS_DTYPE_F32)
+            w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+          else
+            w = make_uint4(fp8_out2<OT>(v[0], v[1]), fp8_out2<OT>(v[2], v[3]), fp8_out2<OT>(v[4], v[5]),
+                           fp8_out2<OT>(v[6], v[7]));
+          *reinterpret_cast<uint4*>(piece(lane, c / PER)) = w;
+        }
       }
       if (whole) {
         fence_proxy_async_smem();
@@ -813,10 +793,17 @@ __global__ void __launch_bounds__(f8::THREADS, 1)
 #pragma unroll
         for (int j = 0; j < PART / 32; j++) bias[j * 32 + lane] = __ushort_as_half(b16[j]);
         __syncwarp();
+#pragma unroll
+        for (int j = 0; j < PART; j += 2) {
+          // columns j, j + 1 of the row; of fragments, pair j / 2: half, 8 columns, upper or lower 8 rows
+          const int col = FRAG ? j / 4 % (PART / 8) * 8 + (lane & 3) * 2 : j;
+          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(bias + col));
+          acc[j] += b.x;
+          acc[j + 1] += b.y;
+        }
       }
       if (__all_sync(0xffffffffu, ok))
-        fp8_write<OT, PART, FRAG>(args, &tmap_o, tma_out, stages, turn, args.bias ? bias : nullptr, ti.row0 + mine, ti.row_end, n,
-                            acc);
+        fp8_write<OT, PART, FRAG>(args, &tmap_o, tma_out, stages, turn, ti.row0 + mine, ti.row_end, n, acc);
     }
     if (lane == 0) bulk_wait();
   }
