@@ -59,6 +59,20 @@ __device__ __forceinline__ __half2 fp8_pair(uint16_t c) {
 }
 __device__ __forceinline__ float fp8_value(uint8_t c) { return __low2float(fp8_pair(c)); }
 
+// The larger magnitude of each half of a pair of 16-bit values (a NaN gives
+// way), and the halves as f32.
+template <int DT>
+__device__ __forceinline__ uint32_t fp8_mag_max2(uint32_t a, uint32_t b) {
+  if constexpr (DT == TS_DTYPE_F16) {
+    const __half2 m = __hmax2(__habs2(*reinterpret_cast<__half2*>(&a)), __habs2(*reinterpret_cast<__half2*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __nv_bfloat162 m =
+        __hmax2(__habs2(*reinterpret_cast<__nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<__nv_bfloat162*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+}
+
 // 16 values of a row (or column) of type DT: eight lanes hold one block of 128.
 template <int DT>
 struct Fp8Piece {
