@@ -34,6 +34,13 @@
 //                half (w - 4) / 4 of the tile's columns; writes the tile.
 //                They take the registers that the others do not need.
 // All waits are bounded (ts_common.cuh) and set the device error flag.
+//
+// What bounds it: the tensor core stands still while TMEM is read, 128 KB for
+// each 128 x 256 x 128; at 8192^3 the MMAs with their copies alone take 373 us,
+// with TMEM read beside them 485, all of it 545 (2.0 PFLOP/s, back to back on
+// one B200; 2.95 and 2.27 for the others).  At k = 640 a tile's output is 2,500
+// of its 8,300 cycles: 65,536 x 1152 x 640 takes 78 us, 128 experts' 262,144 x
+// 1280 x 640 400 us (1.07 PFLOP/s).
 #include "ts_fp8.cuh"
 #include "ts_kernels.h"
 
@@ -371,8 +378,9 @@ __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
 // row size has them, and leave by one TMA store where all 32 rows are this
 // tile's (tma: out can be mapped), else row by row, consecutive lanes on
 // consecutive columns.  (Measured at 65,536 x 1152 x 640: 80 us; the four warps
-// of a column half behind one store of 128 rows 88 us; whole lines by ordinary
-// stores from shared memory 98 us.)
+// of a column half behind one store of 128 rows 88 us; the stores issued by a
+// warp of their own 83 us; whole lines by ordinary stores from shared memory
+// 98 us.)
 template <int OT, int PART, bool FRAG>
 __device__ __forceinline__ void fp8_write(const Fp8MmArgs& a, const CUtensorMap* tmap_o, bool tma, uint8_t* stages,
                                           uint32_t& turn, uint32_t row, uint32_t row_end, uint32_t n,

@@ -3,6 +3,11 @@
 //
 // With a = max |x| over the finite values of a block: s = max(a * (1/448),
 // 2^-100), r = 1/s, code = e4m3(x * r), every f32 step rounded to nearest.
+//
+// DRAM bounds both: every value is read once and every code written once.  By
+// rows 65,536 x 640 fp16 takes 22 us (5.7 of the 6.55 TB/s that a copy
+// reaches), by columns 16,391 x 1280 bf16 14.0 us (4.5 TB/s: a column's codes
+// start inside a sector, so part of each is fetched).
 #include "ts_fp8.cuh"
 #include "ts_kernels.h"
 
@@ -191,8 +196,9 @@ cudaError_t launch_fp8_quant_cols(const Fp8QuantArgs& a, cudaStream_t st) {
 
 cudaError_t launch_fp8_transpose(const uint8_t* codes, uint64_t ldw, const float* scales, uint32_t E, uint32_t N,
                                  uint32_t K, uint8_t* codes_t, uint64_t ldt, float* scales_t, cudaStream_t st) {
-  const uint32_t k_tiles = (K + 63) / 64;
-  const dim3 grid((N + 63) / 64 * k_tiles, E);
+  const uint32_t k_tiles = K / 64 + (K % 64 != 0), n_tiles = N / 64 + (N % 64 != 0);
+  if ((uint64_t)n_tiles * k_tiles > 0x7fffffffu) return cudaErrorInvalidValue;
+  const dim3 grid(n_tiles * k_tiles, E);
   fp8_transpose_kernel<<<grid, 256, 0, st>>>(codes, ldw, scales, N, K, codes_t, ldt, scales_t, k_tiles);
   return cudaGetLastError();
 }
