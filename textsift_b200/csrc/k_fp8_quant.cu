@@ -24,9 +24,9 @@ __global__ void __launch_bounds__(256, 8) fp8_quant_rows_kernel(const Fp8QuantAr
   pdl_trigger();
   pdl_wait();
   const uint32_t nb = fp8_blocks(a.cols), lane = threadIdx.x & 31;
-  const uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const uint64_t row = i / nb * 4 + (lane >> 3);
-  const uint32_t b = (uint32_t)(i % nb), c = b * kFp8Block + (lane & 7) * 16;
+  const uint32_t i = blockIdx.x * 8 + (threadIdx.x >> 5), quad = i / nb;  // below 2^32 (launcher)
+  const uint64_t row = (uint64_t)quad * 4 + (lane >> 3);
+  const uint32_t b = i - quad * nb, c = b * kFp8Block + (lane & 7) * 16;
   if (row >= a.rows) return;
   Fp8Piece<DT> p;
   p.load(reinterpret_cast<const typename Fp8Type<DT>::T*>(a.x) + row * a.ldx, c, a.cols, vec);
@@ -101,11 +101,20 @@ __global__ void __launch_bounds__(256, qc::BLOCKS)
   pdl_trigger();
   pdl_wait();
   uint32_t turn = 0;
-  if (blockIdx.x < tiles) fp8_cols_load<DT>(a, vec, blockIdx.x / col_tiles, blockIdx.x % col_tiles * COLS, tile[0]);
+  // block of rows and tile of columns; a step over the grid is the same pair each time
+  uint32_t next_b = blockIdx.x / col_tiles, next_c = blockIdx.x % col_tiles;
+  const uint32_t step_b = gridDim.x / col_tiles, step_c = gridDim.x % col_tiles;
+  if (blockIdx.x < tiles) fp8_cols_load<DT>(a, vec, next_b, next_c * COLS, tile[0]);
   for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, turn ^= 1) {
-    const uint32_t b = t / col_tiles, c0 = t % col_tiles * COLS, next = t + gridDim.x;
-    if (next < tiles) {
-      fp8_cols_load<DT>(a, vec, next / col_tiles, next % col_tiles * COLS, tile[turn ^ 1]);
+    const uint32_t b = next_b, c0 = next_c * COLS;
+    next_b += step_b;
+    next_c += step_c;
+    if (next_c >= col_tiles) {
+      next_c -= col_tiles;
+      next_b++;
+    }
+    if (t + gridDim.x < tiles) {
+      fp8_cols_load<DT>(a, vec, next_b, next_c * COLS, tile[turn ^ 1]);
       asm volatile("cp.async.wait_group 1;" ::: "memory");
     } else {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -174,7 +183,7 @@ static uint32_t fp8_vec(const Fp8QuantArgs& a) {
 
 cudaError_t launch_fp8_quant_rows(const Fp8QuantArgs& a, cudaStream_t st) {
   const uint64_t warps = ((uint64_t)a.rows + 3) / 4 * fp8_blocks(a.cols), grid = (warps + 7) / 8;
-  if (grid > 0x7fffffffu) return cudaErrorInvalidValue;
+  if (grid > 0x1fffffffu) return cudaErrorInvalidValue;
   const dim3 g((uint32_t)grid), t(256);
   if (a.dtype == TS_DTYPE_F16) return launch_pdl(fp8_quant_rows_kernel<TS_DTYPE_F16>, g, t, 0, st, a, fp8_vec(a));
   if (a.dtype == TS_DTYPE_BF16) return launch_pdl(fp8_quant_rows_kernel<TS_DTYPE_BF16>, g, t, 0, st, a, fp8_vec(a));
