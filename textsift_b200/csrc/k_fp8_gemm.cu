@@ -872,13 +872,16 @@ static cudaError_t launch_gemm_out(const CUtensorMap& ta, const CUtensorMap& tw,
 }
 
 // K = 0: bias or zero (+ what out holds) on the rows that a segment covers.
+constexpr uint32_t kFp8EmptyBlocks = 4096;
+// a block's step past the last row stays in 32 bits
+static_assert(kFp8MaxSize <= 0xffffffffu - kFp8EmptyBlocks, "rows of an empty sum");
 template <int OT>
 __global__ void __launch_bounds__(256) fp8_empty_sum_kernel(const Fp8MmArgs a) {
   using D = Fp8Type<OT>;
   for (uint32_t e = 0; e < a.E; e++) {
-    const int lo = a.seg ? min(max(a.seg[e], 0), (int)a.M) : 0;
-    const int hi = a.seg ? min(max(a.seg[e + 1], 0), (int)a.M) : (int)a.M;
-    for (int m = lo + (int)blockIdx.x; m < hi; m += gridDim.x)
+    const uint32_t lo = a.seg ? (uint32_t)min(max(a.seg[e], 0), (int)a.M) : 0;
+    const uint32_t hi = a.seg ? (uint32_t)min(max(a.seg[e + 1], 0), (int)a.M) : a.M;
+    for (uint32_t m = lo + blockIdx.x; m < hi; m += gridDim.x)
       for (uint32_t n = threadIdx.x; n < a.N; n += 256) {
         auto* o = reinterpret_cast<typename D::T*>(a.out) + (uint64_t)m * a.ldo + n;
         float v = a.bias ? __half2float(reinterpret_cast<const __half*>(a.bias)[(uint64_t)e * a.N + n]) : 0.0f;
@@ -890,7 +893,7 @@ __global__ void __launch_bounds__(256) fp8_empty_sum_kernel(const Fp8MmArgs a) {
 
 cudaError_t launch_fp8_matmul(const Fp8MmArgs& a, cudaStream_t st) {
   if (a.K == 0) {
-    const uint32_t grid = std::min(a.M, 4096u);
+    const uint32_t grid = std::min(a.M, kFp8EmptyBlocks);
     if (a.out_dtype == TS_DTYPE_F16) fp8_empty_sum_kernel<TS_DTYPE_F16><<<grid, 256, 0, st>>>(a);
     else if (a.out_dtype == TS_DTYPE_BF16) fp8_empty_sum_kernel<TS_DTYPE_BF16><<<grid, 256, 0, st>>>(a);
     else fp8_empty_sum_kernel<TS_DTYPE_F32><<<grid, 256, 0, st>>>(a);

@@ -88,7 +88,7 @@ int ts_cuda_op_matmul_fp8(const uint8_t* d_a, uint64_t lda, const float* d_as, u
   if (E == 0 || (E > 1 && !d_seg)) return fp8_fail(TS_ERR_ARG, "%s: E must be 1 without segments", me);
   if (w_block == 1 && (E != 1 || d_seg)) return fp8_fail(TS_ERR_ARG, "%s: w_block 1 takes no segments", me);
   if (E > 1024) return fp8_fail(TS_ERR_UNSUPPORTED, "%s: more than 1024 experts", me);
-  if (M > 0x7fffff00u || N > 0x7fffff00u || K > 0x7fffff00u || (uint64_t)E * N > 0x7fffff00u)
+  if (M > ts::kFp8MaxSize || N > ts::kFp8MaxSize || K > ts::kFp8MaxSize || (uint64_t)E * N > ts::kFp8MaxSize)
     return fp8_fail(TS_ERR_UNSUPPORTED, "%s: sizes must stay below 2^31", me);
   if (M == 0 || N == 0) return TS_OK;
   if (!d_out || (K && (!d_a || !d_as || !d_w || !d_ws))) return fp8_fail(TS_ERR_ARG, "%s: null pointer", me);
@@ -117,7 +117,7 @@ int ts_cuda_op_matvec_fp8(const void* d_x, int32_t x_dtype, uint64_t ldx, const 
   if (!is_float(x_dtype) || !is_float(out_dtype))
     return fp8_fail(TS_ERR_ARG, "%s: x_dtype and out_dtype must be F16, BF16 or F32", me);
   if (M > ts::kFp8MatvecRows) return fp8_fail(TS_ERR_UNSUPPORTED, "%s: at most %u rows", me, ts::kFp8MatvecRows);
-  if (N > 0x7fffff00u || K > 0x7fffff00u) return fp8_fail(TS_ERR_UNSUPPORTED, "%s: sizes must stay below 2^31", me);
+  if (N > ts::kFp8MaxSize || K > ts::kFp8MaxSize) return fp8_fail(TS_ERR_UNSUPPORTED, "%s: sizes must stay below 2^31", me);
   if (M == 0 || N == 0) return TS_OK;
   if (!d_out || (K && (!d_x || !d_w || !d_ws))) return fp8_fail(TS_ERR_ARG, "%s: null pointer", me);
   if (ldx < K || ldo < N) return fp8_fail(TS_ERR_ARG, "%s: rows of x or out overlap", me);

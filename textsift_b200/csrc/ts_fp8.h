@@ -10,6 +10,7 @@ namespace ts {
 
 constexpr uint32_t kFp8Block = 128;       // values that share a scale
 constexpr uint32_t kFp8MatvecRows = 16;   // largest M of the single-token form
+constexpr uint32_t kFp8MaxSize = 0x7fffff00u;  // largest M, N, K and E N of the products
 __host__ __device__ constexpr uint32_t fp8_blocks(uint32_t n) { return n / kFp8Block + (n % kFp8Block != 0); }
 
 // Error flag of the kernels of this file on the current device (bounded waits
