@@ -109,7 +109,7 @@ struct Fp8Piece {
   // values i .. i + 15 of a row of n, zeros past its end
   __device__ __forceinline__ void load(const typename Fp8Type<DT>::T* x, uint32_t i, uint32_t n, bool vec) {
     using T = typename Fp8Type<DT>::T;
-    if (vec && i + 16 <= n) {
+    if (vec && fp8_whole(i, n)) {
       constexpr int PER = 16 / (int)sizeof(T);
 #pragma unroll
       for (int j = 0; j < 16 / PER; j++) {

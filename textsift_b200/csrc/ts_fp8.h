@@ -12,6 +12,11 @@ constexpr uint32_t kFp8Block = 128;       // values that share a scale
 constexpr uint32_t kFp8MatvecRows = 16;   // largest M of the single-token form
 constexpr uint32_t kFp8MaxSize = 0x7fffff00u;  // largest M, N, K and E N of the products
 __host__ __device__ constexpr uint32_t fp8_blocks(uint32_t n) { return n / kFp8Block + (n % kFp8Block != 0); }
+// Values i .. i + 15 all lie below n, any n: i + 16 may not fit 32 bits.
+__host__ __device__ constexpr bool fp8_whole(uint32_t i, uint32_t n) { return i < n && n - i >= 16; }
+static_assert(fp8_whole(0, 16) && !fp8_whole(0, 15) && !fp8_whole(16, 16) && !fp8_whole(0xfffffff0u, 0xffffffffu) &&
+                  fp8_whole(0xffffffe0u, 0xffffffffu),
+              "ends of rows");
 
 // Error flag of the kernels of this file on the current device (bounded waits
 // that ran out), in device memory; null when it cannot be looked up.
