@@ -409,9 +409,13 @@ int ts_cuda_op_router_balance(const void* d_logits, int32_t dtype, uint64_t ldl,
                               float* d_loss, void* d_grad, uint64_t ldg, void* d_work, size_t work_bytes,
                               void* stream);
 
-/* Synchronize `stream` and report the error flag of the operators above on
- * the current device as TS_ERR_DEVICE (a bounded wait that ran out; the flag
- * is cleared), like ts_cuda_check for the operators of a handle. */
+/* Synchronize `stream` and report, as TS_ERR_DEVICE, a bounded wait of the
+ * operators above that ran out on the current device (their outputs are then
+ * incomplete), like ts_cuda_check for the operators of a handle.  The error
+ * flag is the device's, not the stream's: after such an error every stream's
+ * next check returns TS_ERR_DEVICE once, whichever stream the operator ran on
+ * (a graph may replay on another than it was captured on), so no check takes
+ * an error away from another stream's. */
 int ts_cuda_op_check(void* stream);
 
 /* ---- expert parallelism (BASELINE config[4]'s expert-parallel variant; the
@@ -460,6 +464,9 @@ int ts_cuda_ep_plan(const int32_t* counts, const int32_t* recv_counts, int32_t w
  * stays usable.  d_result (device, 2 x i32, may be NULL) receives 1 for each
  * of the two waits that completed normally, 0 for each that gave up. */
 int ts_cuda_selftest_wait_timeout(ts_cuda_t* h, uint32_t limit_us, int32_t* d_result, void* stream);
+/* The same with the error flag that ts_cuda_op_check reports, on the current
+ * device. */
+int ts_cuda_selftest_op_wait_timeout(uint32_t limit_us, int32_t* d_result, void* stream);
 
 /* YaRN RoPE tables of the handle (browser/inference/rope.ts:117-135), fp16
  * [rows, head_dim/2] each, copied to host. */

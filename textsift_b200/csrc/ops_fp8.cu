@@ -3,10 +3,13 @@
 // them allocates or synchronizes.
 #include "textsift_cuda.h"
 #include "ts_fp8.h"
+#include "ts_kernels.h"
 #include "ts_simt.h"
 
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
+#include <unordered_map>
 
 namespace {
 
@@ -30,6 +33,24 @@ bool is_float(int32_t dtype) {
 }
 size_t float_bytes(int32_t dtype) { return dtype == TS_DTYPE_F32 ? 4 : 2; }
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// The error flag is one for a device and all its streams, so whichever check
+// finds it set cannot tell whose work failed.  Errors found are counted, and
+// every stream is told of those it has not heard of.  A flag raised between
+// the copy and the clearing below is not lost either: it belongs to the error
+// that is counted after them, before its own stream can check.
+struct OpErrors {
+  std::mutex lock;
+  struct Device {
+    uint64_t found = 0;
+    std::unordered_map<unsigned long long, uint64_t> told;  // by stream id; only streams that were told of any
+  };
+  std::unordered_map<int, Device> devices;
+};
+OpErrors& op_errors() {
+  static OpErrors* e = new OpErrors;  // checks at exit may come after static destructors
+  return *e;
+}
 
 // Codes of rows of `cols` values, ld bytes apart.
 int check_codes(const char* what, const uint8_t* codes, uint64_t ld, uint32_t cols) {
@@ -164,16 +185,37 @@ int ts_cuda_op_check(void* stream) {
   const char* me = "ts_cuda_op_check";
   cudaStream_t st = (cudaStream_t)stream;
   int* flag = ts::fp8_err_flag();
-  int err = 0;
+  int err = 0, dev = 0;
+  unsigned long long id = 0;
   if (!flag) return fp8_fail(TS_ERR_CUDA, "%s: no error flag on this device", me);
-  cudaError_t e = cudaMemcpyAsync(&err, flag, 4, cudaMemcpyDeviceToHost, st);
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaStreamGetId(st, &id);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);  // before the lock: others need not wait for this stream
+  if (e != cudaSuccess) return fp8_done(me, e);
+  OpErrors& errors = op_errors();
+  std::lock_guard<std::mutex> hold(errors.lock);
+  OpErrors::Device& d = errors.devices[dev];
+  e = cudaMemcpyAsync(&err, flag, 4, cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e == cudaSuccess && err) {
     e = cudaMemsetAsync(flag, 0, 4, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    if (e == cudaSuccess) return fp8_fail(TS_ERR_DEVICE, "device error flag %d (bounded wait timed out)", err);
+    if (e == cudaSuccess) d.found++;
   }
-  return fp8_done(me, e);
+  if (e != cudaSuccess) return fp8_done(me, e);
+  const auto heard = d.told.find(id);
+  if (d.found == (heard == d.told.end() ? 0 : heard->second)) return TS_OK;
+  d.told[id] = d.found;
+  return fp8_fail(TS_ERR_DEVICE, "%s: device error flag (bounded wait timed out) on a stream of this device", me);
+}
+
+int ts_cuda_selftest_op_wait_timeout(uint32_t limit_us, int32_t* d_result, void* stream) {
+  const char* me = "ts_cuda_selftest_op_wait_timeout";
+  if (limit_us == 0 || limit_us > 1000000u) return fp8_fail(TS_ERR_ARG, "%s: limit_us must be in [1, 1000000]", me);
+  if (!aligned(d_result, 4)) return fp8_fail(TS_ERR_ARG, "%s: d_result must be aligned to its type", me);
+  int* flag = ts::fp8_err_flag();
+  if (!flag) return fp8_fail(TS_ERR_CUDA, "%s: no error flag on this device", me);
+  return fp8_done(me, ts::launch_wait_selftest(flag, 1000ull * limit_us, d_result, (cudaStream_t)stream));
 }
 
 }  // extern "C"
