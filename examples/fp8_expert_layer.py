@@ -61,8 +61,10 @@ class Weight:
         full = torch.zeros(e, _up(n, BLOCK), _up(k, BLOCK), device="cuda")
         full[:, :n, :k] = w
         v = full.view(e, full.shape[1] // BLOCK, BLOCK, full.shape[2] // BLOCK, BLOCK)
-        self.scales = (v.abs().amax((2, 4)) / 448.0).clamp_min(2.0 ** -100).contiguous()
-        q = (v / self.scales[:, :, None, :, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+        # the format's roundings: the scale is the largest magnitude times f32(1/448), the codes are those of v times
+        # the scale's f32 reciprocal
+        self.scales = (v.abs().amax((2, 4)) * (1.0 / 448.0)).clamp_min(2.0 ** -100).contiguous()
+        q = (v * (1.0 / self.scales)[:, :, None, :, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
         self.codes = torch.zeros(e, n, _up(k, 16), dtype=torch.uint8, device="cuda")
         self.codes[:, :, :k] = q.view(e, full.shape[1], full.shape[2])[:, :n, :k].view(torch.uint8)
         self.codes_t = torch.zeros(e, k, _up(n, 16), dtype=torch.uint8, device="cuda")
