@@ -144,7 +144,7 @@ def step(x: torch.Tensor, router: torch.Tensor, gate_up: Weight, down: Weight, s
     for e in range(down.e):
         if ends[e + 1] > ends[e]:
             grad_weight(droutes[ends[e]:ends[e + 1]], g[ends[e]:ends[e + 1]], dw[e])
-    return {"y": y, "loss": loss, "counts": counts, "prob": prob, "dlogits": dlogits, "seg": seg, "order": order, "g": g,
+    return {"y": y, "routes": routes, "weight": weight.flatten()[order], "loss": loss, "counts": counts, "prob": prob, "dlogits": dlogits, "seg": seg, "order": order, "g": g,
             "dg": dg, "dw": dw, "droutes": droutes}
 
 
@@ -168,19 +168,24 @@ def main(argv=None) -> dict:
     # the same in f32 on the weights that the codes stand for
     seg, token = out["seg"].tolist(), out["order"] // a.k
     wu, wd = gate_up.value(), down.value()
-    err = {"forward": 0.0, "input gradient": 0.0, "weight gradient": 0.0}
+    err = {"forward": 0.0, "down product": 0.0, "input gradient": 0.0, "weight gradient": 0.0}
+    y = torch.zeros(x.shape, device="cuda")
     for e in range(a.experts):
         r = slice(seg[e], seg[e + 1])
         if seg[e] == seg[e + 1]:
             continue
         g = swiglu((x[token[r]].float() @ wu[e].t()).half())
+        routes = out["g"][r].float() @ wd[e].t()
+        y.index_add_(0, token[r], routes * out["weight"][r, None])
         pairs = {"forward": (out["g"][r].float(), g.float()),
+                 "down product": (out["routes"][r].float(), routes),
                  "input gradient": (out["dg"][r].float(), out["droutes"][r].float() @ wd[e]),
                  "weight gradient": (out["dw"][e], out["droutes"][r].float().t() @ out["g"][r].float())}
         for name, (got, want) in pairs.items():
             err[name] = max(err[name], float((got - want).norm() / want.norm()))
+    err["output"] = float((out["y"] - y).norm() / y.norm())
     print(f"{a.tokens} tokens, {a.experts} experts: balance loss {float(out['loss']):.6f}, routes per expert "
-          f"{int(out['counts'].sum(0).min())}..{int(out['counts'].sum(0).max())}; largest error of an expert against f32: "
+          f"{int(out['counts'].sum(0).min())}..{int(out['counts'].sum(0).max())}; largest errors against f32: "
           + ", ".join(f"{n} {v:.3f}" for n, v in err.items()))
     return {**out, "errors": err}
 
