@@ -469,6 +469,14 @@ int ts_cuda_selftest_wait_timeout(ts_cuda_t* h, uint32_t limit_us, int32_t* d_re
 /* The same with the error flag that ts_cuda_op_check reports, on the current
  * device. */
 int ts_cuda_selftest_op_wait_timeout(uint32_t limit_us, int32_t* d_result, void* stream);
+/* Which kernel form ts_cuda_op_matmul_fp8 takes for these sizes (segments != 0:
+ * with d_seg) on a GPU of `sms` streaming multiprocessors (0: the current
+ * device's), so that tests know what they reach.  The choice is an estimate of
+ * time, not part of the interface.  0: K = 0; 1: single tokens; 2: CTA pairs
+ * on 256 x 256 tiles; 3, 4: single CTAs on 128 x 128, 128 x 64; 5, 6, 7: 2, 4,
+ * 8 CTAs share a tile's k.  Host only; negative: TS_ERR_ARG. */
+int ts_cuda_selftest_matmul_fp8_form(uint32_t M, uint32_t N, uint32_t K, int32_t w_block, int32_t segments, uint32_t E,
+                                     uint32_t sms);
 
 /* YaRN RoPE tables of the handle (browser/inference/rope.ts:117-135), fp16
  * [rows, head_dim/2] each, copied to host. */

@@ -106,6 +106,7 @@ SIGNATURES = [
     ("ts_cuda_ep_plan", ctypes.c_int, [P, P, I32, I32, I32, P, P, P, U32, P]),
     ("ts_cuda_selftest_wait_timeout", ctypes.c_int, [P, U32, P, P]),
     ("ts_cuda_selftest_op_wait_timeout", ctypes.c_int, [U32, P, P]),
+    ("ts_cuda_selftest_matmul_fp8_form", ctypes.c_int, [U32, U32, U32, I32, I32, U32, U32]),
     # host tokenizer
     ("ts_tok_create", P, [ctypes.c_char_p, ctypes.c_size_t, ctypes.c_char_p, ctypes.c_size_t]),
     ("ts_tok_destroy", None, [P]),

@@ -891,15 +891,61 @@ __global__ void __launch_bounds__(256) fp8_empty_sum_kernel(const Fp8MmArgs a) {
   }
 }
 
+// Tiles of bm rows: exact without segments; with them, an upper bound of what
+// M rows in E segments can make.
+static uint64_t fp8_m_tiles(const Fp8MmArgs& a, uint32_t bm) {
+  return a.seg ? a.M / bm + std::min(a.E, a.M) : ((uint64_t)a.M + bm - 1) / bm;
+}
+
+// The form with the shortest estimate: rounds of tiles over the SMs, each
+// `chunk` us for 128 of k (w_block 128, 1) and `tile` for the rest; the CTAs
+// of a split do not outlive their tile, so a second round costs them a start.
+// Measured, us, [pairs, 128, 64, 128 / 2, 128 / 4] at w_block 128:
+//   8192 x 8192 x 8192   [546, 726, 1228, -, -]   1024 x 1024 x 8192  [40, 29, 27, 21, 27]
+//   2048 x 2048 x 2048   [16, 19, 28, -, -]       128 x 4096 x 4096   [22, 16, 15, 14, 10]
+//   512 x 640 x 640      [8.7, 6.8, 5.8, -, -]
+// and 1280 x 640 x 16384 at w_block 1 [117, 80, -, 47, 53].
+struct Fp8Tiling {
+  Fp8Form form;
+  uint32_t cg, bn, split;
+  double chunk[2], tile;
+};
+static constexpr Fp8Tiling kFp8Tilings[] = {
+    {Fp8Form::pairs, 2, 256, 1, {0.60, 0.92}, 1.1},   {Fp8Form::wide, 1, 128, 1, {0.40, 0.60}, 1.0},
+    {Fp8Form::narrow, 1, 64, 1, {0.35, 0}, 0.6},      {Fp8Form::split2, 1, 128, 2, {0.40, 0.60}, 3.5},
+    {Fp8Form::split4, 1, 128, 4, {0.40, 0.60}, 3.5},  {Fp8Form::split8, 1, 128, 8, {0.40, 0.60}, 3.5}};
+
+static const Fp8Tiling* fp8_tiling(const Fp8MmArgs& a, uint64_t sms) {
+  const uint64_t n_kc = fp8_blocks(a.K);
+  const Fp8Tiling* best = nullptr;
+  double least = 0.0;
+  for (const Fp8Tiling& f : kFp8Tilings) {
+    if (f.split > n_kc || (f.bn < 128 && a.w_block == 1)) continue;
+    const uint64_t tiles = fp8_m_tiles(a, f.cg * f8::BM) * ((a.N + f.bn - 1) / f.bn), at_once = sms / (f.cg * f.split);
+    const uint64_t rounds = (tiles + at_once - 1) / at_once, chunks = (n_kc + f.split - 1) / f.split;
+    const double us = (double)rounds * ((double)chunks * f.chunk[a.w_block == 1] + f.tile) +
+                      (f.split > 1 ? (double)(rounds - 1) * 3.5 : 0.0);
+    if (!best || us < least) best = &f, least = us;
+  }
+  return best;
+}
+
+Fp8Form fp8_matmul_form(const Fp8MmArgs& a, uint32_t sms) {
+  if (a.K == 0) return Fp8Form::empty;
+  if (a.M <= kFp8MatvecRows && a.w_block != 1 && !a.seg) return Fp8Form::matvec;
+  return fp8_tiling(a, sms)->form;
+}
+
 cudaError_t launch_fp8_matmul(const Fp8MmArgs& a, cudaStream_t st) {
-  if (a.K == 0) {
+  const Fp8Form form = fp8_matmul_form(a, (uint32_t)num_sms());
+  if (form == Fp8Form::empty) {
     const uint32_t grid = std::min(a.M, kFp8EmptyBlocks);
     if (a.out_dtype == TS_DTYPE_F16) fp8_empty_sum_kernel<TS_DTYPE_F16><<<grid, 256, 0, st>>>(a);
     else if (a.out_dtype == TS_DTYPE_BF16) fp8_empty_sum_kernel<TS_DTYPE_BF16><<<grid, 256, 0, st>>>(a);
     else fp8_empty_sum_kernel<TS_DTYPE_F32><<<grid, 256, 0, st>>>(a);
     return cudaGetLastError();
   }
-  if (a.M <= kFp8MatvecRows && a.w_block != 1 && !a.seg) {
+  if (form == Fp8Form::matvec) {
     Fp8MvArgs v;
     v.x = a.a; v.x_dtype = TS_DTYPE_U8; v.ldx = a.lda; v.xs = a.as; v.ldxs = a.ldas; v.w = a.w; v.ldw = a.ldw;
     v.ws = a.ws; v.bias = a.bias; v.out = a.out; v.out_dtype = a.out_dtype; v.ldo = a.ldo; v.accumulate = a.accumulate;
@@ -910,41 +956,14 @@ cudaError_t launch_fp8_matmul(const Fp8MmArgs& a, cudaStream_t st) {
   if (!make_codes_tmap(&ta, a.a, a.M, a.K, a.lda, f8::BM) ||
       !make_codes_tmap(&tw, a.w, (uint64_t)a.E * a.N, a.K, a.ldw, f8::W_BOX))
     return cudaErrorInvalidValue;
-  // tiles of bm rows: exact without segments; with them, an upper bound of what
-  // M rows in E segments can make
-  auto m_tiles = [&](uint32_t bm) { return a.seg ? a.M / bm + std::min(a.E, a.M) : ((uint64_t)a.M + bm - 1) / bm; };
-  // The form with the shortest estimate: rounds of tiles over the SMs, each
-  // `chunk` us for 128 of k (w_block 128, 1) and `tile` for the rest; the CTAs
-  // of a split do not outlive their tile, so a second round costs them a start.
-  // Measured, us, [pairs, 128, 64, 128 / 2, 128 / 4] at w_block 128:
-  //   8192 x 8192 x 8192   [546, 726, 1228, -, -]   1024 x 1024 x 8192  [40, 29, 27, 21, 27]
-  //   2048 x 2048 x 2048   [16, 19, 28, -, -]       128 x 4096 x 4096   [22, 16, 15, 14, 10]
-  //   512 x 640 x 640      [8.7, 6.8, 5.8, -, -]
-  // and 1280 x 640 x 16384 at w_block 1 [117, 80, -, 47, 53].
-  const uint64_t sms = (uint64_t)num_sms(), n_kc = fp8_blocks(a.K);
-  struct Form {
-    uint32_t cg, bn, split;
-    double chunk[2], tile;
-  };
-  static constexpr Form forms[] = {{2, 256, 1, {0.60, 0.92}, 1.1}, {1, 128, 1, {0.40, 0.60}, 1.0}, {1, 64, 1, {0.35, 0}, 0.6},
-                                   {1, 128, 2, {0.40, 0.60}, 3.5}, {1, 128, 4, {0.40, 0.60}, 3.5},
-                                   {1, 128, 8, {0.40, 0.60}, 3.5}};
-  const Form* best = nullptr;
-  double least = 0.0;
-  for (const Form& f : forms) {
-    if (f.split > n_kc || (f.bn < 128 && a.w_block == 1)) continue;
-    const uint64_t tiles = m_tiles(f.cg * f8::BM) * ((a.N + f.bn - 1) / f.bn), at_once = sms / (f.cg * f.split);
-    const uint64_t rounds = (tiles + at_once - 1) / at_once, chunks = (n_kc + f.split - 1) / f.split;
-    const double us = (double)rounds * ((double)chunks * f.chunk[a.w_block == 1] + f.tile) +
-                      (f.split > 1 ? (double)(rounds - 1) * 3.5 : 0.0);
-    if (!best || us < least) best = &f, least = us;
+  switch (form) {
+    case Fp8Form::pairs: return launch_gemm_out<2, 256, false>(ta, tw, a, fp8_m_tiles(a, 2 * f8::BM), 1, st);
+    case Fp8Form::wide: return launch_gemm_out<1, 128, false>(ta, tw, a, fp8_m_tiles(a, f8::BM), 1, st);
+    case Fp8Form::narrow: return launch_gemm_out<1, 64, false>(ta, tw, a, fp8_m_tiles(a, f8::BM), 1, st);
+    case Fp8Form::split2: return launch_gemm_out<1, 128, true>(ta, tw, a, fp8_m_tiles(a, f8::BM), 2, st);
+    case Fp8Form::split4: return launch_gemm_out<1, 128, true>(ta, tw, a, fp8_m_tiles(a, f8::BM), 4, st);
+    default: return launch_gemm_out<1, 128, true>(ta, tw, a, fp8_m_tiles(a, f8::BM), 8, st);
   }
-  const uint64_t mt = m_tiles(best->cg * f8::BM);
-  if (best->cg == 2) return launch_gemm_out<2, 256, false>(ta, tw, a, mt, 1, st);
-  if (best->bn == 128)
-    return best->split == 1 ? launch_gemm_out<1, 128, false>(ta, tw, a, mt, 1, st)
-                            : launch_gemm_out<1, 128, true>(ta, tw, a, mt, best->split, st);
-  return launch_gemm_out<1, 64, false>(ta, tw, a, mt, 1, st);
 }
 
 }  // namespace ts

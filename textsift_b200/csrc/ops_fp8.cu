@@ -131,6 +131,18 @@ int ts_cuda_op_matmul_fp8(const uint8_t* d_a, uint64_t lda, const float* d_as, u
   return fp8_done(me, ts::launch_fp8_matmul(a, (cudaStream_t)stream));
 }
 
+int ts_cuda_selftest_matmul_fp8_form(uint32_t M, uint32_t N, uint32_t K, int32_t w_block, int32_t segments, uint32_t E,
+                                     uint32_t sms) {
+  const char* me = "ts_cuda_selftest_matmul_fp8_form";
+  if (M == 0 || N == 0 || E == 0) return fp8_fail(TS_ERR_ARG, "%s: sizes must be positive", me);
+  if (w_block != 128 && w_block != 1) return fp8_fail(TS_ERR_ARG, "%s: w_block must be 128 or 1", me);
+  if (sms != 0 && sms < 8) return fp8_fail(TS_ERR_ARG, "%s: sms must be 0 or 8 at least", me);
+  ts::Fp8MmArgs a;
+  static const int some[1] = {0};  // stands for segments, which are not read
+  a.M = M; a.N = N; a.K = K; a.w_block = w_block; a.seg = segments ? some : nullptr; a.E = E;
+  return (int)ts::fp8_matmul_form(a, sms ? sms : (uint32_t)ts::num_sms());
+}
+
 int ts_cuda_op_matvec_fp8(const void* d_x, int32_t x_dtype, uint64_t ldx, const uint8_t* d_w, uint64_t ldw,
                           const float* d_ws, const uint16_t* d_bias, void* d_out, int32_t out_dtype, uint64_t ldo,
                           uint32_t M, uint32_t N, uint32_t K, void* stream) {

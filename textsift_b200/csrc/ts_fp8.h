@@ -58,6 +58,11 @@ struct Fp8MmArgs {
   int* err = nullptr;
 };
 cudaError_t launch_fp8_matmul(const Fp8MmArgs& a, cudaStream_t st);
+// What that launches on a GPU of `sms` (8 or more) SMs, by sizes, w_block and segments
+// alone: the sum of nothing, the single-token form, CTA pairs on 256 x 256
+// tiles, single CTAs on 128 x 128 or 128 x 64, clusters that split k.
+enum class Fp8Form { empty, matvec, pairs, wide, narrow, split2, split4, split8 };
+Fp8Form fp8_matmul_form(const Fp8MmArgs& a, uint32_t sms);
 
 // x of a floating type, quantised on the way, or codes (x_dtype TS_DTYPE_U8)
 // with their scales xs.
