@@ -51,14 +51,6 @@ __device__ __forceinline__ uint32_t fp8_codes2(float x0, float x1, float r) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(__fmul_rn(x1, r)), "f"(__fmul_rn(x0, r)));
   return c;
 }
-// The two values of a pair of codes, exact in fp16.
-__device__ __forceinline__ __half2 fp8_pair(uint16_t c) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
-  return *reinterpret_cast<__half2*>(&h);
-}
-__device__ __forceinline__ float fp8_value(uint8_t c) { return __low2float(fp8_pair(c)); }
-
 // The larger magnitude of each half of a pair of 16-bit values (a NaN gives
 // way), and the halves as f32.
 template <int DT>
