@@ -359,11 +359,13 @@ int ts_cuda_op_transpose_fp8(const uint8_t* d_codes, uint64_t ldw, const float* 
  *   w_block 1: d_w, ldw, d_ws, ldws a row operand [N, K], E = 1 (a weight
  *     gradient: a = dY transposed, w = X transposed, K the tokens);
  *   d_bias: fp16 [E][N] or NULL;
- *   d_seg: NULL (E = 1: every row by the one weight), or i32 [E + 1]: rows
- *     [seg[e], seg[e+1]) are multiplied with expert e's weight; rows outside
- *     every segment are not written, bounds are clamped to [0, M];
+ *   d_seg: NULL (E = 1: every row by the one weight), or i32 [E + 1],
+ *     ascending: rows [seg[e], seg[e+1]) are multiplied with expert e's weight;
+ *     rows outside every segment are not written, bounds are clamped to [0, M];
  *   d_out: out_dtype TS_DTYPE_F16, BF16 or F32, [M, N], ldo elements between
- *     rows; accumulate != 0 (F32 only) adds to what d_out holds. */
+ *     rows; accumulate != 0 (F32 only) adds to what d_out holds.
+ * A block's two scales are multiplied with each other first, in f32, so that
+ * product has to be in f32's normal range where its codes are not zero. */
 int ts_cuda_op_matmul_fp8(const uint8_t* d_a, uint64_t lda, const float* d_as, uint64_t ldas, const uint8_t* d_w,
                           uint64_t ldw, const float* d_ws, uint64_t ldws, int32_t w_block, const uint16_t* d_bias,
                           const int32_t* d_seg, uint32_t E, void* d_out, int32_t out_dtype, uint64_t ldo,

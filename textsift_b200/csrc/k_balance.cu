@@ -17,9 +17,9 @@
 // Large calls run as four launches (clear, count, tokens, loss), small ones
 // as one block that keeps counts and sums in shared memory: there the chain
 // of launches and of global round trips is all that costs.  65,536 x 128 f32
-// over 44 documents takes 28 us (clear 2, count 6, tokens 19, loss 6, partly
-// at once; 10.4 us at the copy's rate), 80 x 128 7.4 us a call, the host's time
-// for one (17 us as five launches).
+// over 44 documents takes 28.2 us (clear 2, count 6, tokens 19, loss 6, partly
+// at once; 10.4 us at the copy's rate), 80 x 128 7.0 to 7.5 us a call, the host's
+// time for one (17 us as five launches).
 #include "ts_fp8.cuh"
 #include "ts_kernels.h"
 

@@ -33,14 +33,22 @@
 //   warps 4..11  scale and add: warp w owns TMEM lanes 32 (w % 4).. (rows) and
 //                half (w - 4) / 4 of the tile's columns; writes the tile.
 //                They take the registers that the others do not need.
-// All waits are bounded (ts_common.cuh) and set the device error flag.
+// The waits on mbarriers are bounded (ts_common.cuh) and set the device error
+// flag.  The cluster barriers and the TMEM allocation have no limit of their
+// own and need none: every thread of a cluster comes to each barrier after its
+// bounded waits, whether they succeeded or not, and a block takes 64,512 of the
+// SM's 65,536 registers, so no kernel of this library that takes TMEM for
+// longer than a bounded wait is on the SM beside it.
 //
 // What bounds it: the tensor core stands still while TMEM is read, 128 KB for
 // each 128 x 256 x 128; at 8192^3 the MMAs with their copies alone take 373 us,
-// with TMEM read beside them 485, all of it 545 (2.0 PFLOP/s, back to back on
-// one B200; 2.95 and 2.27 for the others).  At k = 640 a tile's output is 2,500
-// of its 8,300 cycles: 65,536 x 1152 x 640 takes 78 us, 128 experts' 262,144 x
-// 1280 x 640 400 us (1.07 PFLOP/s).
+// with TMEM read beside them 485, all of it 539 to 545 (2.0 PFLOP/s; 2.95 and
+// 2.27 for the others).  At k = 640 a tile's output is 2,500 of its 8,300
+// cycles: 65,536 x 1152 x 640 takes 82 us, with a bias 100, 128 experts' 262,144
+// x 1280 x 640 378 us (1.14 PFLOP/s).  These are times of one call repeated on
+// the same inputs, on one B200; with inputs that change from call to call
+// 8192^3 takes 622 us (power), 65,536 x 1152 x 640 with a bias 96, the experts
+// 426.
 #include "ts_fp8.cuh"
 #include "ts_kernels.h"
 
@@ -377,7 +385,8 @@ __device__ __forceinline__ uint32_t fp8_out2(float x0, float x1) {
 // while the other leaves, their 16-byte pieces swizzled as a tensor map of that
 // row size has them, and leave by one TMA store where all 32 rows are this
 // tile's (tma: out can be mapped), else row by row, consecutive lanes on
-// consecutive columns.  (Measured at 65,536 x 1152 x 640: 80 us; the four warps
+// consecutive columns.  (Measured at 65,536 x 1152 x 640 without bias, one call
+// repeated: 80 us; the four warps
 // of a column half behind one store of 128 rows 88 us; the stores issued by a
 // warp of their own 83 us; whole lines by ordinary stores from shared memory
 // 98 us.)
@@ -900,7 +909,8 @@ static uint64_t fp8_m_tiles(const Fp8MmArgs& a, uint32_t bm) {
 // The form with the shortest estimate: rounds of tiles over the SMs, each
 // `chunk` us for 128 of k (w_block 128, 1) and `tile` for the rest; the CTAs
 // of a split do not outlive their tile, so a second round costs them a start.
-// Measured, us, [pairs, 128, 64, 128 / 2, 128 / 4] at w_block 128:
+// Measured, us a call repeated on the same inputs, [pairs, 128, 64, 128 / 2,
+// 128 / 4] at w_block 128:
 //   8192 x 8192 x 8192   [546, 726, 1228, -, -]   1024 x 1024 x 8192  [40, 29, 27, 21, 27]
 //   2048 x 2048 x 2048   [16, 19, 28, -, -]       128 x 4096 x 4096   [22, 16, 15, 14, 10]
 //   512 x 640 x 640      [8.7, 6.8, 5.8, -, -]

@@ -4,10 +4,12 @@
 // With a = max |x| over the finite values of a block: s = max(a * (1/448),
 // 2^-100), r = 1/s, code = e4m3(x * r), every f32 step rounded to nearest.
 //
-// DRAM bounds both: every value is read once and every code written once.  By
-// rows 65,536 x 640 fp16 takes 22 us (5.7 of the 6.55 TB/s that a copy
-// reaches), by columns 16,391 x 1280 bf16 14.0 us (4.5 TB/s: a column's codes
-// start inside a sector, so part of each is fetched).
+// Every value is read once and every code written once.  By rows 65,536 x 640
+// fp16 takes 22.5 us (5.7 of the 6.55 TB/s that a copy reaches; a warp issues
+// in 68% of the cycles), by columns 16,391 x 1280 bf16 13.9 us (4.6 TB/s):
+// there instructions bound it, 74% of the issue slots, with DRAM at 31% and
+// nothing read but the input.  (Times of calls whose input changes from one to
+// the next.)
 #include "ts_fp8.cuh"
 #include "ts_kernels.h"
 
